@@ -86,6 +86,11 @@ SIGNATURES = {
     "sm_scan_chunk": "ii" "plplplplpl" "pppp" "ppp" "iii" "ff",
     "sm_thin_gemm": "iplpppliiii" "piii",
     "sm_thin_act": "iplppp" "iiiiiiiii" "ffff",
+    "sm_mx_quantize": "iplppii",
+    "sm_mx_dequantize": "ipppii",
+    "sm_mx_linear": "iplppppiii",
+    "sm_mx_grad": "iplpppiii",
+    "sm_mx_matmul": "ippppppiii",
 }
 
 

@@ -1,0 +1,311 @@
+"""The MXFP4 kernels against float64 at the edges of their tiles: every pattern of the 16-bit types, rows and columns that end
+inside a tile, k that ends inside a stage, strided rows, non-finite rows, graphs and streams."""
+import pytest
+import torch
+
+import _ref_mxfp4 as ref
+from lumen.ops.mxfp4 import MXFP4, mxfp4_dequantize, mxfp4_linear, mxfp4_matmul, mxfp4_quantize
+
+pytestmark = pytest.mark.gpu
+HALF = [torch.bfloat16, torch.float16]
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(seed, *shape):
+    return torch.randn(*shape, device="cuda", generator=gen(seed))
+
+
+def weight(seed, N, K, spread=1.0):
+    """A weight [N, K] whose blocks differ in size, in MXFP4, and its values in float64."""
+    w = randn(seed, N, K) * 0.05 * torch.exp(spread * randn(seed + 1, N, K // 32)).repeat_interleave(32, 1)
+    q = mxfp4_quantize(w.bfloat16())
+    return q, ref.values(q)
+
+
+# ---- the format -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", HALF)
+def test_every_pattern(dtype):
+    """Each of the 65536 values in a block whose largest is 2^0 ... 2^3 times as large: all codes, ties and denormals."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16)
+    v = bits.view(dtype)
+    v = v[torch.isfinite(v.float())]
+    v = v[:len(v) // 16 * 16].view(-1, 16)
+    v = v[torch.randperm(len(v), generator=torch.Generator().manual_seed(0))]
+    block = torch.cat((v, v.flip(0)), 1)                  # two runs of neighbouring values of different size
+    same = torch.cat((v, v), 1)
+    x = torch.cat((block, same)).contiguous()
+    q = mxfp4_quantize(x.cuda())
+    code, byte = ref.encode(x)
+    got = ref.unpack(q)
+    assert torch.equal(got[1], byte) and torch.equal(got[0], code)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, *HALF])
+@pytest.mark.parametrize("R,K", [(1, 32), (1, 4096), (3, 96), (5, 416), (70, 2048), (257, 160), (4, 11008)])
+def test_quantize(R, K, dtype):
+    x = (randn(R + K, R, K + 24) * torch.exp(3 * randn(K, R, 1))).clamp(-6e4, 6e4).to(dtype)[:, 8:8 + K]
+    code, byte = ref.encode(x)
+    for rows in (x, x.contiguous(), x.t().contiguous().t()):
+        q = mxfp4_quantize(rows)
+        got = ref.unpack(q)
+        assert torch.equal(got[1], byte) and torch.equal(got[0], code)
+        assert int(q._codes[:, K // 2:].sum()) == 0 and int(q._scales[:, K // 32:].sum()) == 0
+    want = ref.decode(code, byte)
+    for dt in (torch.float32, torch.bfloat16, torch.float16):
+        assert torch.equal(mxfp4_dequantize(q, dt).cpu(), want.to(dt))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, *HALF])
+def test_non_finite_blocks(dtype):
+    x = randn(1, 4, 128).to(dtype)
+    x[0, 33], x[1, 0], x[2, 127] = float("inf"), float("nan"), -float("inf")
+    x[3, :32] = 0
+    q = mxfp4_quantize(x)
+    code, byte = ref.encode(x)
+    assert torch.equal(ref.unpack(q)[0], code) and torch.equal(ref.unpack(q)[1], byte)
+    y = mxfp4_dequantize(q, dtype)
+    assert torch.isnan(y[0, 32:64]).all() and torch.isnan(y).sum() == 96
+    y = mxfp4_matmul(q, mxfp4_quantize(randn(2, 20, 128)), out_dtype=torch.float32)
+    assert torch.isnan(y[:3]).all() and torch.isfinite(y[3]).all()
+
+
+def test_all_codes_and_scales_dequantize():
+    code = torch.arange(256, dtype=torch.uint8).view(16, 16).repeat(256, 1)           # 32 codes a row
+    scale = torch.arange(256, dtype=torch.uint8).view(256, 1).repeat_interleave(16, 0)
+    q = MXFP4(code.cuda(), scale.cuda())
+    want = ref.values(q)
+    for dt in (torch.float32, torch.bfloat16, torch.float16):
+        got = mxfp4_dequantize(q, dt).cpu()
+        assert torch.equal(torch.nan_to_num(got, nan=1234.0), torch.nan_to_num(want.to(dt), nan=1234.0))
+
+
+# ---- products -------------------------------------------------------------------------------------
+ROWS = [1, 2, 3, 4, 7, 8, 9, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 100, 127, 128, 129, 200, 255, 256, 257, 300, 513]
+SIZES = [(1, 32), (4, 64), (15, 96), (16, 128), (20, 160), (33, 224), (66, 416), (130, 512), (257, 704), (520, 1056)]
+
+
+def check_linear(M, N, K, dtype, bias, seed=0, wide=True):
+    x = randn(M * 7 + N + K + seed, M, K + (16 if wide else 0)).to(dtype)[:, (8 if wide else 0):][:, :K]
+    q, _ = weight(N + K, N, K)
+    W = mxfp4_dequantize(q, dtype).double().cpu()
+    b = randn(N, N).to(dtype) if bias else None
+    xd = x.double().cpu()
+    want, mag = xd @ W.t(), xd.abs() @ W.abs().t()
+    if bias:
+        want, mag = want + b.double().cpu(), mag + b.double().cpu().abs()
+    y = mxfp4_linear(x, q, b)
+    assert y.dtype == dtype and y.shape == (M, N) and y.is_contiguous()
+    ref.close(y, want, mag, K + 1, dtype)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M", ROWS)
+def test_linear_rows(M, dtype):
+    for i, (N, K) in enumerate(SIZES):
+        check_linear(M, N, K, dtype, bias=i % 2 == 0, wide=i % 3 == 0)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (5, 1000, 5632), (17, 2048, 2048), (64, 4100, 1024), (96, 1028, 4128), (509, 1000, 2080),
+                                   (1021, 2048, 544), (2050, 516, 1024), (1030, 4097, 288)])
+def test_linear_sizes(M, N, K, dtype):
+    check_linear(M, N, K, dtype, bias=True)
+
+
+def check_grad(M, N, K, dtype, wide=False):
+    dy = randn(M * 3 + N + K, M, N + (16 if wide else 0)).to(dtype)[:, (8 if wide else 0):][:, :N]
+    q, _ = weight(N + K, N, K)
+    W = mxfp4_dequantize(q, dtype).double().cpu()
+    x = randn(1, M, K).to(dtype).requires_grad_()
+    y = mxfp4_linear(x, q)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    assert dx.dtype == dtype and dx.shape == (M, K)
+    d = dy.double().cpu()
+    ref.close(dx, d @ W, d.abs() @ W.abs(), N, dtype)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M", ROWS)
+def test_grad_rows(M, dtype):
+    for i, (N, K) in enumerate(SIZES):
+        check_grad(M, N, K, dtype, wide=i % 3 == 0)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,N,K", [(1, 2048, 4096), (509, 1000, 2080), (300, 1001, 1024), (1021, 544, 2048), (2050, 1030, 544), (64, 4096, 1024)])
+def test_grad_sizes(M, N, K, dtype):
+    check_grad(M, N, K, dtype)
+
+
+def check_matmul(M, N, K, dtype, bias):
+    a = mxfp4_quantize((randn(M + K, M, K) * torch.exp(randn(K, M, 1))).bfloat16())
+    b, B = weight(N + K, N, K)
+    A = ref.values(a)
+    c = randn(N, N).to(dtype) if bias else None
+    want, mag = A @ B.t(), A.abs() @ B.abs().t()
+    if bias:
+        want, mag = want + c.double().cpu(), mag + c.double().cpu().abs()
+    y = mxfp4_matmul(a, b, bias=c, out_dtype=dtype)
+    assert y.dtype == dtype and y.shape == (M, N)
+    ref.close(y, want, mag, K + 1, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, *HALF])
+@pytest.mark.parametrize("M", ROWS)
+def test_matmul_rows(M, dtype):
+    for i, (N, K) in enumerate(SIZES):
+        check_matmul(M, N, K, dtype, bias=i % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,N,K", [(1, 2048, 4096), (48, 4100, 5632), (509, 1000, 2080), (1021, 2048, 544), (2050, 516, 1024), (1030, 4097, 288)])
+def test_matmul_sizes(M, N, K, dtype):
+    check_matmul(M, N, K, dtype, bias=True)
+
+
+@pytest.mark.parametrize("M", [3, 64, 300])
+def test_scales_from_the_smallest_to_the_largest(M):
+    """Products whose scales cancel: rows of 2^100 against weights of 2^-100, blocks far below their neighbours."""
+    x = randn(1, M, 256).bfloat16()
+    big = (x.float() * 2.0 ** 100).bfloat16()
+    w = randn(2, 80, 256)
+    q = mxfp4_quantize((w * 2.0 ** -100).bfloat16())
+    W = ref.values(q)
+    ref.close(mxfp4_linear(big, q), big.double().cpu() @ W.t(), big.double().cpu().abs() @ W.abs().t(), 256, torch.bfloat16)
+    a = mxfp4_quantize(big)
+    A = ref.values(a)
+    ref.close(mxfp4_matmul(a, q, out_dtype=torch.float32), A @ W.t(), A.abs() @ W.abs().t(), 256, torch.float32)
+
+
+@pytest.mark.parametrize("M", [2, 33, 140, 300])
+@pytest.mark.parametrize("K", [128, 160])
+def test_non_finite_rows_stay_theirs(M, K):
+    """An infinite or missing value of a row reaches that row alone; an infinite one keeps its sign where no other meets it."""
+    x = randn(3, M, K).bfloat16()
+    q, _ = weight(5, 70, K)
+    clean = mxfp4_linear(x, q)
+    x[0, K - 1], x[1, 3] = float("inf"), float("nan")
+    y = mxfp4_linear(x, q)
+    assert torch.equal(y[2:], clean[2:])
+    W = mxfp4_dequantize(q, torch.float32)
+    want = x.float() @ W.t()
+    assert torch.equal(torch.isnan(y[:2]), torch.isnan(want[:2]))
+    inf = torch.isinf(want[0])
+    assert torch.equal(y[0][inf].float(), want[0][inf])
+
+
+@pytest.mark.parametrize("M", [5, 300])
+def test_memory_around_the_rows_is_left_alone(M):
+    """Rows in a buffer of NaN: nothing beside them is read into a result."""
+    for K in (160, 128):
+        buf = torch.full((M + 2, K + 64), float("nan"), device="cuda", dtype=torch.bfloat16)
+        x = buf[1:M + 1, 32:32 + K]
+        x.copy_(randn(1, M, K))
+        q, _ = weight(7, 50, K)
+        assert torch.equal(mxfp4_linear(x, q), mxfp4_linear(x.contiguous(), q))
+        assert torch.isfinite(mxfp4_dequantize(mxfp4_quantize(x))).all()
+
+
+def test_leading_dimensions_and_odd_strides():
+    q, _ = weight(3, 40, 96)
+    x = randn(1, 2, 5, 96).bfloat16()
+    y = mxfp4_linear(x, q)
+    assert y.shape == (2, 5, 40)
+    assert torch.equal(y.view(10, 40), mxfp4_linear(x.view(10, 96), q))
+    odd = torch.zeros(10, 97, device="cuda", dtype=torch.bfloat16)[:, 1:]
+    odd.copy_(x.view(10, 96))
+    assert torch.equal(mxfp4_linear(odd, q), y.view(10, 40))
+    t = x.view(10, 96).t().contiguous().t()
+    assert torch.equal(mxfp4_linear(t, q), y.view(10, 40))
+    one = x.view(10, 96)[:1].expand(10, 96)               # a row read ten times
+    assert torch.equal(mxfp4_linear(one, q), y.view(10, 40)[:1].expand(10, 40))
+
+
+def test_a_run_as_a_layer_makes_it():
+    """Quantised base, rows through it, the gradient back, against the same in float64; then with 4-bit rows."""
+    w = randn(1, 300, 256) * 0.05
+    x = randn(2, 70, 256).bfloat16()
+    q = mxfp4_quantize(w.bfloat16())
+    leaf = x.clone().requires_grad_()
+    y = mxfp4_linear(leaf, q)
+    (y.float() ** 2).sum().backward()
+    W = ref.values(q)
+    dy = 2 * y.detach().double().cpu()
+    rounded = dy.to(torch.bfloat16).double()
+    ref.close(leaf.grad, rounded @ W, rounded.abs() @ W.abs(), 300, torch.bfloat16)
+    a = mxfp4_quantize(x)
+    z = mxfp4_matmul(a, q)
+    ref.close(z, ref.values(a) @ W.t(), ref.values(a).abs() @ W.abs().t(), 256, torch.bfloat16)
+
+
+@pytest.mark.parametrize("M", [1, 40, 400])
+def test_captured_calls_replay_on_new_rows(M):
+    q, _ = weight(1, 500, 288)
+    x = randn(1, M, 288).bfloat16()
+    dy = randn(2, M, 500).bfloat16()
+    from lumen.ops.mxfp4 import _input_grad
+
+    def step():
+        return mxfp4_linear(x, q), mxfp4_matmul(mxfp4_quantize(x), q), _input_grad(dy, q)
+
+    step()
+    torch.cuda.synchronize()
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+    with torch.cuda.graph(other):
+        z = step()
+    for i in range(4):
+        x.copy_(randn(10 + i, M, 288))
+        dy.copy_(randn(20 + i, M, 500))
+        want = step()
+        graph.replay()
+        other.replay()
+        torch.cuda.synchronize()
+        for a, b, c in zip(want, y, z):
+            assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_another_stream():
+    q, _ = weight(1, 260, 512)
+    x = randn(1, 90, 512).bfloat16()
+    want = mxfp4_linear(x, q), mxfp4_matmul(mxfp4_quantize(x), q)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = mxfp4_linear(x, q), mxfp4_matmul(mxfp4_quantize(x), q)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_the_same_call_gives_the_same_bits():
+    q, _ = weight(1, 1000, 2048)
+    for M in (1, 30, 300):
+        x = randn(M, M, 2048).bfloat16()
+        assert torch.equal(mxfp4_linear(x, q), mxfp4_linear(x, q))
+
+
+def test_refused_on_the_gpu():
+    q, _ = weight(1, 16, 64)
+    x = randn(1, 3, 64)
+    for f in (lambda: mxfp4_linear(x, q), lambda: mxfp4_linear(x.cpu().bfloat16(), q), lambda: mxfp4_linear(x.bfloat16(), q, torch.zeros(16).bfloat16()),
+              lambda: mxfp4_matmul(mxfp4_quantize(x.cpu()), q)):
+        with pytest.raises(ValueError):
+            f()
+
+
+def test_empty_on_the_gpu():
+    q, _ = weight(1, 16, 64)
+    x = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = mxfp4_linear(x, q)
+    assert y.shape == (0, 16)
+    (dx,) = torch.autograd.grad(y.sum(), x)
+    assert dx.shape == (0, 64)
+    e = mxfp4_quantize(x)
+    assert e.shape == (0, 64) and mxfp4_matmul(e, q).shape == (0, 16) and mxfp4_dequantize(e).shape == (0, 64)
+    x = randn(1, 3, 64).bfloat16().requires_grad_()
+    (dx,) = torch.autograd.grad(mxfp4_linear(x, e).sum(), x)
+    assert mxfp4_matmul(q, e).shape == (16, 0) and int(dx.abs().sum()) == 0
