@@ -1,0 +1,80 @@
+// dx = dy w of 16-bit rows and an MXFP4 weight, on tiles (mx_loop.h).
+#include "mx_tile.h"
+
+using namespace lumen;
+using mx::TileArgs;
+
+namespace {
+
+template <typename T, int MJ, int WN>
+__global__ void __launch_bounds__(256, 1) grad_kernel(const TileArgs a) {
+  using S = mx::Shape<8, MJ, WN, true>;
+  __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tm, tn;
+  tile::tile_at(tile::unit_of(blockIdx.x, gridDim.x), a.tiles_m, a.tiles_n, a.group, tm, tn);
+  const int m0 = tm * S::BM, panel = tn * WN, panels = (a.K + 127) / 128;
+  const int nk = (a.N + 63) / 64, left = a.N - 64 * (nk - 1);
+  const long long wp = (long long)a.N * 64, sp = (long long)a.N * 4;
+  unsigned offx[S::PX], offw[S::PW], lastw[S::PW];
+#pragma unroll
+  for (int q = 0; q < S::PX; ++q) {
+    const int r = 8 * (wid + 4 * q) + (lane >> 3);
+    offx[q] = (unsigned)min(r, a.M - m0 - 1) * (unsigned)(2 * a.ldx) + 16 * ((lane & 7) ^ tile::swz(r));
+  }
+#pragma unroll
+  for (int q = 0; q < S::PW; ++q) {
+    const int pc = (wid + 4 * q) % S::NW, pos = 16 * (pc & 1) + (lane >> 2);
+    const int n = 32 * ((pc >> 1) & 1) + ((pos & 3) << 3 | pos >> 2);
+    const unsigned at = (unsigned)min(pc >> 2, panels - 1 - panel) * (unsigned)wp + 16 * (lane & 3);
+    offw[q] = at + 64 * n;
+    lastw[q] = at + 64 * min(n, left - 1);
+  }
+  const unsigned as = (unsigned)min(wid % WN, panels - 1 - panel) * (unsigned)sp;
+  const mx::Walk walk{(const char*)a.x + (long long)m0 * a.ldx * 2, (const char*)a.codes + panel * wp, (const char*)a.scales + panel * sp,
+                      wp, sp, nk, a.Nx - 64 * (nk - 1), left};
+  f32x4 acc[8][MJ];
+  mx::products<T, 8, MJ, WN, true>(lds, walk, offx, offw, as + 4 * lane, lastw, as + 4 * min(lane, left - 1), acc);
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    const int m = m0 + 16 * MJ * (wid / WN) + 16 * j + lr;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx::hold<mx::kNamed<8, MJ>>(acc[i][j]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {                        // row 4 lg + e of fragment i: column 8 (4 lg + e) + i
+      const int k = 128 * (panel + wid % WN) + 32 * lg + 8 * e;
+      const float r[8] = {acc[0][j][e], acc[1][j][e], acc[2][j][e], acc[3][j][e], acc[4][j][e], acc[5][j][e], acc[6][j][e], acc[7][j][e]};
+      if (m < a.M && k < a.K) store8((T*)a.y + (long long)m * a.K + k, r);
+    }
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+// dx [M, K] = dy [M, N] w; dy 16-bit at ldy, its rows readable (and zero) up to a multiple of 8 values; tiles of 64 mj / wn x 128 wn
+hipError_t sm_mx_grad(int dt, const void* dy, long long ldy, const void* codes, const void* scales, void* dx, int M, int N, int K, int mj,
+                      int wn, hipStream_t st) {
+  const int Nx = (N + 7) / 8 * 8;
+  if (!mx::sizes_ok(M, N, K) || ldy < Nx || ldy % 8 || ldy > (1 << 22) || ((uintptr_t)dx | (uintptr_t)dy | (uintptr_t)codes | (uintptr_t)scales) % 16 ||
+      (dt != kF16 && dt != kBF16))
+    return hipErrorInvalidValue;
+  TileArgs a{dy, ldy, nullptr, codes, scales, nullptr, dx, M, N, K, Nx, 0, 0, 0, 8};
+  int grid;
+  if (!mx::plan(a, K, 64 * mj / wn, 128 * wn, grid)) return hipErrorInvalidValue;
+  switch (10 * mj + wn) {
+#define GO(MJ, WN)                                                                     \
+  case 10 * MJ + WN:                                                                   \
+    if (dt == kBF16) grad_kernel<bf16, MJ, WN><<<grid, 256, 0, st>>>(a);               \
+    else grad_kernel<fp16, MJ, WN><<<grid, 256, 0, st>>>(a);                           \
+    break;
+    GO(1, 1) GO(2, 1) GO(4, 1) GO(1, 2) GO(2, 2) GO(4, 2) GO(8, 2)
+#undef GO
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // extern "C"

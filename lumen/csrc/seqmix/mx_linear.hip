@@ -1,0 +1,63 @@
+// y = x w^T + bias of 16-bit rows and an MXFP4 weight, on tiles (mx_loop.h).
+#include "mx_tile.h"
+
+using namespace lumen;
+using mx::TileArgs;
+
+namespace {
+
+template <typename T, int NI, int MJ, int WN>
+__global__ void __launch_bounds__(256, 1) linear_kernel(const TileArgs a) {
+  using S = mx::Shape<NI, MJ, WN, false>;
+  __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tm, tn;
+  tile::tile_at(tile::unit_of(blockIdx.x, gridDim.x), a.tiles_m, a.tiles_n, a.group, tm, tn);
+  const int m0 = tm * S::BM, n0 = tn * S::BN;
+  auto column = [&](int r) { return min(n0 + r / (16 * NI) * (16 * NI) + tile::colperm<NI>(r % (16 * NI)), a.N - 1); };
+  unsigned offx[S::PX], offw[S::PW], offs;
+#pragma unroll
+  for (int q = 0; q < S::PX; ++q) {                      // (rows past the edge read the last row: never stored)
+    const int r = 8 * (wid + 4 * q) + (lane >> 3);
+    offx[q] = (unsigned)min(r, a.M - m0 - 1) * (unsigned)(2 * a.ldx) + 16 * ((lane & 7) ^ tile::swz(r));
+  }
+#pragma unroll
+  for (int q = 0; q < S::PW; ++q)
+    offw[q] = (unsigned)column((wid + 4 * q) % S::NW * 32 + (lane & 31)) * 64u + 16 * (lane >> 5);
+  offs = (unsigned)column(min(64 * wid + lane, S::BN - 1)) * 4u;
+  const int nk = (a.K + 63) / 64;
+  const mx::Walk walk{(const char*)a.x + (long long)m0 * a.ldx * 2, (const char*)a.codes, (const char*)a.scales, (long long)a.N * 64,
+                      (long long)a.N * 4, nk, a.K - 64 * (nk - 1), 64};
+  f32x4 acc[NI][MJ];
+  mx::products<T, NI, MJ, WN, false>(lds, walk, offx, offw, offs, offw, offs, acc);
+  mx::put_all<T, NI, MJ>(a, acc, m0 + 16 * MJ * (wid / WN), n0 + 16 * NI * (wid % WN));
+}
+
+}  // namespace
+
+extern "C" {
+
+// y [M, N] = x [M, K] w^T + bias (or null), x 16-bit at ldx, 16-byte aligned rows; tiles of 32 mj x 32 ni
+hipError_t sm_mx_linear(int dt, const void* x, long long ldx, const void* codes, const void* scales, const void* bias, void* y,
+                        int M, int N, int K, int mj, int ni, hipStream_t st) {
+  if (!mx::sizes_ok(M, N, K) || ldx < K || ldx % 8 || ldx > (1 << 22) || ((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) % 16 ||
+      (dt != kF16 && dt != kBF16))
+    return hipErrorInvalidValue;
+  TileArgs a{x, ldx, nullptr, codes, scales, bias, y, M, N, K, 0, 0, 0, 0, mx::store_width(y, N, 2)};
+  int grid;
+  if (!mx::plan(a, N, 32 * mj, 32 * ni, grid)) return hipErrorInvalidValue;
+  switch (10 * mj + ni) {
+#define GO(MJ, NI)                                                                     \
+  case 10 * MJ + NI:                                                                   \
+    if (dt == kBF16) linear_kernel<bf16, NI, MJ, 2><<<grid, 256, 0, st>>>(a);          \
+    else linear_kernel<fp16, NI, MJ, 2><<<grid, 256, 0, st>>>(a);                      \
+    break;
+    GO(1, 1) GO(1, 2) GO(1, 4) GO(1, 8) GO(2, 1) GO(2, 2) GO(2, 4) GO(2, 8) GO(4, 2) GO(4, 4) GO(4, 8) GO(8, 2) GO(8, 4) GO(8, 6) GO(8, 8)
+#undef GO
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // extern "C"

@@ -1,0 +1,356 @@
+// Main loops of products with MXFP4 weights on tiles, one workgroup of four waves per CU.
+//
+// Rows in MXFP4 lie in panels of 128 k: codes [K / 128][rows][64 bytes], scales [K / 128][rows][4 bytes] (mxfp4.hip), so that a stage
+// of a tile is one run of memory whichever product reads it.
+//  * Operands come by LDS-DMA, as many stages ahead as fit into 160 KiB, under counted waits; one barrier a stage.
+//  * While the matrix core multiplies one set of fragments, the next set is read and made: between two products stands at most a
+//    read, a DMA or a few instructions of the vector unit, which the matrix core's 16 cycles cover.
+//  * 192 and more accumulators are named as accumulation registers in the products' assembly: the compiler, left to place them, moves
+//    them to and fro.  It knows nothing of such products' latency, so nothing may read or move an accumulator before settle(): the
+//    loops have one way round and settle before they are left.  Fewer are the compiler's.
+#pragma once
+#include "mx.h"
+#include "../kernels/tile_loop.h"
+
+namespace lumen {
+namespace mx {
+
+constexpr int kLds = 160 * 1024;
+template <int NI, int MJ> constexpr bool kNamed = NI * MJ >= 48;
+
+// c += a b, 16 x 16 x 32
+template <typename T, bool NAMED>
+__device__ __forceinline__ void mfma(f32x4& c, uint4 a, uint4 b) {
+  if constexpr (NAMED) tile::mfma<T>(c, a, b);
+  else c = Mfma<T>::run(a, b, c);
+}
+// the last products have left the matrix core
+template <bool NAMED> __device__ __forceinline__ void settle() { if constexpr (NAMED) tile::settle(); }
+template <bool NAMED> __device__ __forceinline__ void hold(f32x4& c) { if constexpr (NAMED) tile::hold(c); }
+
+// LDS-DMA of 4 bytes per lane
+__device__ __forceinline__ void dma4(const void* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+
+__device__ __forceinline__ unsigned lds_addr(const char* p) {
+  return (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p);
+}
+
+// two 16-bit values of byte W of eight codes, in the place where it is written: a product may follow two instructions later
+template <typename T, int W>
+__device__ __forceinline__ unsigned pair(unsigned c, float scale) {
+  unsigned r;
+  if constexpr (__is_same(T, bf16)) {
+    if constexpr (W == 0) asm volatile("v_cvt_scalef32_pk_bf16_fp4 %0, %1, %2" : "=v"(r) : "v"(c), "v"(scale));
+    if constexpr (W == 1) asm volatile("v_cvt_scalef32_pk_bf16_fp4 %0, %1, %2 op_sel:[1,0,0]" : "=v"(r) : "v"(c), "v"(scale));
+    if constexpr (W == 2) asm volatile("v_cvt_scalef32_pk_bf16_fp4 %0, %1, %2 op_sel:[0,1,0]" : "=v"(r) : "v"(c), "v"(scale));
+    if constexpr (W == 3) asm volatile("v_cvt_scalef32_pk_bf16_fp4 %0, %1, %2 op_sel:[1,1,0]" : "=v"(r) : "v"(c), "v"(scale));
+  } else {
+    if constexpr (W == 0) asm volatile("v_cvt_scalef32_pk_f16_fp4 %0, %1, %2" : "=v"(r) : "v"(c), "v"(scale));
+    if constexpr (W == 1) asm volatile("v_cvt_scalef32_pk_f16_fp4 %0, %1, %2 op_sel:[1,0,0]" : "=v"(r) : "v"(c), "v"(scale));
+    if constexpr (W == 2) asm volatile("v_cvt_scalef32_pk_f16_fp4 %0, %1, %2 op_sel:[0,1,0]" : "=v"(r) : "v"(c), "v"(scale));
+    if constexpr (W == 3) asm volatile("v_cvt_scalef32_pk_f16_fp4 %0, %1, %2 op_sel:[1,1,0]" : "=v"(r) : "v"(c), "v"(scale));
+  }
+  return r;
+}
+
+// what the vector unit wrote is there for the matrix core
+__device__ __forceinline__ void ready() { asm volatile("s_nop 1" ::: "memory"); }
+
+// ---- 16-bit rows against 4-bit weights -------------------------------------------------------------
+//
+// Tiles of 16 MJ WM rows of x and 16 NI WN columns, WM x WN = 4 waves, a wave 16 MJ x 16 NI.  A stage is 64 of the summed index.
+//  * GRAD false: y = x w^T.  A fragment of w is 16 of its rows by 32 k, one block a row: a lane reads four bytes, its 8 codes.
+//  * GRAD true: dx = dy w, the sum runs over w's rows.  A lane takes 8 rows' codes of the 8 columns it stands for; two rows' pairs
+//    are regrouped by column (v_perm), which gives 8 fragments, of columns 8 a + j for j = 0 .. 7 (a: row of the fragment).
+template <int NI, int MJ, int WN, bool GRAD>
+struct Shape {
+  static constexpr int WM = 4 / WN, BM = 16 * MJ * WM, BN = 16 * NI * WN;
+  static constexpr int XB = BM * 128, WB = BN * 32, SB = XB + WB + 1024;      // a stage: x, codes, scales
+  static constexpr int PX = BM / 32, NW = BN / 32, PW = (NW + 3) / 4, PIECES = PX + PW + 1;
+  static constexpr int FIT = kLds / SB, NST = FIT < 6 ? FIT : 6, LDS = NST * SB;
+  static_assert(BM % 32 == 0 && BN % 32 == 0 && BN <= 256 && NST >= 3 && (NST - 1) * PIECES < 64, "tile");
+  static_assert(!GRAD || NI == 8, "a panel a wave");
+};
+
+struct Walk {
+  const char* x;              // first row of the tile, 2-byte elements, 128 bytes a stage
+  const char *w, *s;          // codes and scales: of panel 0 and row 0 (GRAD: of the tile's first panel)
+  long long wp, sp;           // bytes from panel to panel
+  int nk, tail, tailw;        // stages; values of x in the last one (a multiple of 8); GRAD: rows of w in it
+};
+
+// acc[i][j] += products of fragments i of w and j of x.  offx[q], offw[q], offs: the lane's byte offsets of its pieces; lastw, lasts: of
+// those of the last stage (GRAD), whose rows from `tail` on are not w's own.
+template <typename T, int NI, int MJ, int WN, bool GRAD>
+__device__ __forceinline__ void products(char* lds, const Walk& a, const unsigned (&offx)[Shape<NI, MJ, WN, GRAD>::PX],
+                                         const unsigned (&offw)[Shape<NI, MJ, WN, GRAD>::PW], unsigned offs,
+                                         const unsigned (&lastw)[Shape<NI, MJ, WN, GRAD>::PW], unsigned lasts,
+                                         f32x4 (&acc)[NI][MJ]) {
+  using S = Shape<NI, MJ, WN, GRAD>;
+  constexpr bool NAMED = kNamed<NI, MJ>;
+  constexpr int PX = S::PX, PW = S::PW, NW = S::NW, P = S::PIECES, NST = S::NST, SB = S::SB, XB = S::XB, WB = S::WB;
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wid / WN, wn = wid % WN;
+  const unsigned lds0 = lds_addr(lds);
+  const int cx = (lane & 7) ^ ((4 * wid + (lane >> 4)) & 7);             // chunk of x that the lane brings
+  const bool beyond = 8 * cx >= a.tail;
+  const unsigned back = beyond ? 16 * cx : 0;
+  auto issue = [&](int t, int slot, int q0, int q1) __attribute__((always_inline)) {
+    const bool last = t == a.nk - 1;
+    const char* xs = a.x + (long long)t * 128;
+    const char* ws = GRAD ? a.w + (long long)t * 4096 : a.w + (t >> 1) * a.wp + (t & 1) * 32;
+    const char* ss = GRAD ? a.s + (long long)t * 256 : a.s + (t >> 1) * a.sp;
+    const unsigned d = __builtin_amdgcn_readfirstlane(lds0 + slot * SB + wid * 1024);
+#pragma unroll
+    for (int q = q0; q < q1; ++q) {
+      if (q < PX) tile::dma16(xs, offx[q] - (last ? back : 0u), d + q * 4096);
+      else if (q < PX + PW) {
+        const int u = q - PX;
+        const unsigned to = NW % 4 == 0 ? d + XB + u * 4096
+                                        : __builtin_amdgcn_readfirstlane(lds0 + slot * SB + XB + (wid + 4 * u) % NW * 1024);
+        tile::dma16(ws, GRAD && last ? lastw[u] : offw[u], to);
+      } else {
+        dma4(ss, GRAD && last ? lasts : offs, __builtin_amdgcn_readfirstlane(lds0 + slot * SB + XB + WB + wid * 256));
+      }
+    }
+  };
+  // what a last stage holds beyond the sum's end becomes zero; each wave mends the pieces that it sent for
+  auto mend = [&](int slot) __attribute__((always_inline)) {
+    if (a.tail == 64 && (!GRAD || a.tailw == 64)) return;
+    char* d = lds + slot * SB;
+    if (beyond) {
+#pragma unroll
+      for (int q = 0; q < PX; ++q) *reinterpret_cast<uint4*>(d + wid * 1024 + q * 4096 + lane * 16) = make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (GRAD) {
+#pragma unroll
+      for (int u = 0; u < PW; ++u) {
+        const int pc = (wid + 4 * u) % NW, pos = 16 * (pc & 1) + (lane >> 2);
+        if (32 * ((pc >> 1) & 1) + ((pos & 3) << 3 | pos >> 2) >= a.tailw)
+          *reinterpret_cast<uint4*>(d + XB + pc * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
+      }
+      if (lane >= a.tailw) *reinterpret_cast<unsigned*>(d + XB + WB + wid * 256 + lane * 4) = 0;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f}, hold<NAMED>(acc[i][j]);
+  settle<NAMED>();
+  constexpr int RW = GRAD ? 8 : NI;                      // reads of codes of a half
+  uint4 fx[2][MJ];
+  unsigned fw[2][NI][4], raw[RW], sc[RW];
+  float fs[GRAD ? 2 : 1];
+  const int xrow = (16 * MJ * wm + lr) * 128;
+  const int wrow = 16 * NI * wn + lr;
+  // read n of half h of a stage: codes, scales (a row's four, once a stage; GRAD: the byte), fragments of x
+  constexpr int RS = RW, READS = RW + RS + MJ;
+  auto read = [&](int h, int slot, int n) __attribute__((always_inline)) {
+    const char* d = lds + slot * SB;
+    if (n < RW) {
+      if constexpr (GRAD) {
+        raw[n] = *reinterpret_cast<const unsigned*>(d + XB + wn * 4096 + h * 2048 + (4 * n + lg) * 64 + lr * 4);
+      } else {
+        const int r = wrow + 16 * n;
+        raw[n] = *reinterpret_cast<const unsigned*>(d + XB + (r >> 5) * 1024 + h * 512 + (r & 31) * 16 + lg * 4);
+      }
+    } else if (n < RW + RS) {
+      const int u = n - RW;
+      if constexpr (GRAD) sc[u] = *reinterpret_cast<const unsigned char*>(d + XB + WB + wn * 256 + (32 * h + 8 * lg + u) * 4 + (lr >> 2));
+      else if (h == 0) sc[u] = *reinterpret_cast<const unsigned*>(d + XB + WB + (wrow + 16 * u) * 4);
+    } else {
+      const int u = n - RW - RS;
+      fx[h][u] = *reinterpret_cast<const uint4*>(d + xrow + u * 2048 + (((4 * h + lg) ^ tile::swz(16 * MJ * wm + lr)) << 4));
+    }
+  };
+  // unit n of the making of half h's fragments of w; t: their stage
+  constexpr int UNITS = GRAD ? 16 : 4 * NI;
+  auto make = [&](int h, int t, int n) __attribute__((always_inline)) {
+    const int w = n & 3, u = n >> 2;
+    if constexpr (GRAD) {                                // rows 2 u and 2 u + 1, columns 2 w and 2 w + 1
+      if (w == 0) fs[0] = mx_scale(sc[2 * u]), fs[1] = mx_scale(sc[2 * u + 1]);
+      unsigned p, q;
+      if (w == 0) p = pair<T, 0>(raw[2 * u], fs[0]), q = pair<T, 0>(raw[2 * u + 1], fs[1]);
+      else if (w == 1) p = pair<T, 1>(raw[2 * u], fs[0]), q = pair<T, 1>(raw[2 * u + 1], fs[1]);
+      else if (w == 2) p = pair<T, 2>(raw[2 * u], fs[0]), q = pair<T, 2>(raw[2 * u + 1], fs[1]);
+      else p = pair<T, 3>(raw[2 * u], fs[0]), q = pair<T, 3>(raw[2 * u + 1], fs[1]);
+      asm volatile("v_perm_b32 %0, %1, %2, %3" : "=v"(fw[h][2 * w][u]) : "v"(q), "v"(p), "s"(0x05040100u));
+      asm volatile("v_perm_b32 %0, %1, %2, %3" : "=v"(fw[h][2 * w + 1][u]) : "v"(q), "v"(p), "s"(0x07060302u));
+    } else {
+      if (w == 0) fs[0] = mx_scale((sc[u] >> (16 * (t & 1) + 8 * h)) & 255u);
+      if (w == 0) fw[h][u][0] = pair<T, 0>(raw[u], fs[0]);
+      else if (w == 1) fw[h][u][1] = pair<T, 1>(raw[u], fs[0]);
+      else if (w == 2) fw[h][u][2] = pair<T, 2>(raw[u], fs[0]);
+      else fw[h][u][3] = pair<T, 3>(raw[u], fs[0]);
+    }
+  };
+  // the products of half h, between them reads and making of the other half, of stage t2 in `slot`, and send(a, b): pieces a .. b - 1
+  auto half = [&](int h, int t2, int slot, auto&& send) __attribute__((always_inline)) {
+    constexpr int U = NI * MJ, UR = (U * 3 + 7) / 8, UV = U / 4;         // reads in products 0 .. UR - 1, making from UV on
+    ready();
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int n = j * NI + i;
+        mfma<T, NAMED>(acc[i][j], make_uint4(fw[h][i][0], fw[h][i][1], fw[h][i][2], fw[h][i][3]), fx[h][j]);
+#pragma unroll
+        for (int r = min(READS, (n * READS + UR - 1) / UR); r < min(READS, ((n + 1) * READS + UR - 1) / UR); ++r) read(1 - h, slot, r);
+        if (n >= UV) {
+#pragma unroll
+          for (int r = (n - UV) * UNITS / (U - UV); r < (n - UV + 1) * UNITS / (U - UV); ++r) make(1 - h, t2, r);
+        }
+        send(n * P / U, (n + 1) * P / U);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  const auto none = [](int, int) __attribute__((always_inline)) {};
+  const int nk = a.nk;
+#pragma unroll
+  for (int u = 0; u < NST; ++u)
+    if (u < nk) issue(u, u, 0, P);
+  // stage 0 has arrived
+  tile::wait_stages<NST - 1, P>(nk - 1);
+  if (nk == 1) mend(0);
+  tile::done_reading();
+#pragma unroll
+  for (int r = 0; r < READS; ++r) read(0, 0, r);
+#pragma unroll
+  for (int r = 0; r < UNITS; ++r) make(0, 0, r);
+  for (int t = 0, s0 = 0, s1 = 1;;) {                    // slots of stages t and t + 1
+    half(0, t, s0, none);
+    tile::wait_stages<NST - 2, P>(nk - 2 - t);           // stage t + 1 has arrived
+    if (t + 2 == nk) mend(s1);
+    tile::done_reading();
+    const bool more = t + NST < nk;
+    half(1, t + 1, s1, [&](int b, int e) __attribute__((always_inline)) { if (more) issue(t + NST, s0, b, e); });
+    s0 = s1, s1 = s1 == NST - 1 ? 0 : s1 + 1;            // (the last step reads a slot that holds an earlier stage, or none: unused)
+    if (++t == nk) break;
+  }
+  settle<NAMED>();
+}
+
+// ---- both operands in 4 bits ---------------------------------------------------------------------------
+//
+// Tiles as above; a stage is a panel, 128 k: one scaled product of 16 x 16 x 128 per pair of fragments, which takes a block and its scale
+// byte from every lane.
+template <int NI, int MJ, int WN>
+struct Shape4 {
+  static constexpr int WM = 4 / WN, BM = 16 * MJ * WM, BN = 16 * NI * WN;
+  static constexpr int XB = BM * 64, WB = BN * 64, SB = XB + WB + 2048;
+  static constexpr int NX = BM / 16, NW = BN / 16, PX = (NX + 3) / 4, PW = (NW + 3) / 4, PIECES = PX + PW + 2;
+  static constexpr int FIT = kLds / SB, NST = FIT < 6 ? FIT : 6, LDS = NST * SB;
+  static_assert(BM <= 256 && BN <= 256 && NST >= 3 && (NST - 1) * PIECES < 64, "tile");
+};
+
+struct Walk4 {
+  const char *x, *xs, *w, *s;  // codes and scales of both
+  long long xp, xsp, wp, sp;   // bytes from panel to panel
+  int nk;
+};
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+template <bool NAMED>
+__device__ __forceinline__ void mfma4(f32x4& c, uint4 a, uint4 b, unsigned sa, unsigned sb) {
+  if constexpr (NAMED)
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                 : "+a"(c) : "v"(__builtin_bit_cast(u32x4, a)), "v"(__builtin_bit_cast(u32x4, b)), "v"(sa), "v"(sb));
+  else
+    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w},
+                                                         i32x8{(int)b.x, (int)b.y, (int)b.z, (int)b.w}, c, 4, 4, 0, (int)sa, 0, (int)sb);
+}
+
+template <int NI, int MJ, int WN>
+__device__ __forceinline__ void products4(char* lds, const Walk4& a, const unsigned (&offx)[Shape4<NI, MJ, WN>::PX], unsigned offxs,
+                                          const unsigned (&offw)[Shape4<NI, MJ, WN>::PW], unsigned offs, f32x4 (&acc)[NI][MJ]) {
+  using S = Shape4<NI, MJ, WN>;
+  constexpr bool NAMED = kNamed<NI, MJ>;
+  constexpr int PX = S::PX, PW = S::PW, NX = S::NX, NW = S::NW, P = S::PIECES, NST = S::NST, SB = S::SB, XB = S::XB, WB = S::WB;
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wid / WN, wn = wid % WN;
+  const unsigned lds0 = lds_addr(lds);
+  auto issue = [&](int u, int slot, int q0, int q1) __attribute__((always_inline)) {
+    const unsigned d = lds0 + slot * SB;
+    const int t = min(u, a.nk - 1);
+#pragma unroll
+    for (int q = q0; q < q1; ++q) {
+      if (q < PX) tile::dma16(a.x + t * a.xp, offx[q], __builtin_amdgcn_readfirstlane(d + (wid + 4 * q) % NX * 1024));
+      else if (q < PX + PW)
+        tile::dma16(a.w + t * a.wp, offw[q - PX], __builtin_amdgcn_readfirstlane(d + XB + (wid + 4 * (q - PX)) % NW * 1024));
+      else if (q == PX + PW) dma4(a.xs + t * a.xsp, offxs, __builtin_amdgcn_readfirstlane(d + XB + WB + wid * 256));
+      else dma4(a.s + t * a.sp, offs, __builtin_amdgcn_readfirstlane(d + XB + WB + 1024 + wid * 256));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f}, hold<NAMED>(acc[i][j]);
+  settle<NAMED>();
+  uint4 fx[2][MJ], fw[2][NI];
+  unsigned sx[2][MJ], sw[2][NI];
+  const int xrow = 16 * MJ * wm + lr, wrow = 16 * NI * wn + lr;
+  constexpr int READS = 2 * (NI + MJ), UNITS = NI + MJ;
+  auto read = [&](int h, int slot, int n) __attribute__((always_inline)) {
+    const char* d = lds + slot * SB;
+    if (n < NI) sw[h][n] = *reinterpret_cast<const unsigned*>(d + XB + WB + 1024 + (wrow + 16 * n) * 4);
+    else if (n < NI + MJ) sx[h][n - NI] = *reinterpret_cast<const unsigned*>(d + XB + WB + (xrow + 16 * (n - NI)) * 4);
+    else if (n < 2 * NI + MJ) fw[h][n - NI - MJ] = *reinterpret_cast<const uint4*>(d + XB + (wrow + 16 * (n - NI - MJ)) * 64 + lg * 16);
+    else fx[h][n - 2 * NI - MJ] = *reinterpret_cast<const uint4*>(d + (xrow + 16 * (n - 2 * NI - MJ)) * 64 + lg * 16);
+  };
+  auto make = [&](int h, int n) __attribute__((always_inline)) {         // a lane's byte of its row's four
+    if (n < NI) asm volatile("v_lshrrev_b32 %0, %1, %0" : "+v"(sw[h][n]) : "v"(8 * lg));
+    else asm volatile("v_lshrrev_b32 %0, %1, %0" : "+v"(sx[h][n - NI]) : "v"(8 * lg));
+  };
+  auto step = [&](int h, int slot, auto&& send) __attribute__((always_inline)) {
+    constexpr int U = NI * MJ, UR = (U * 5 + 7) / 8, UV = U / 2;
+    ready();
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int n = j * NI + i;
+        mfma4<NAMED>(acc[i][j], fw[h][i], fx[h][j], sw[h][i], sx[h][j]);
+#pragma unroll
+        for (int r = min(READS, (n * READS + UR - 1) / UR); r < min(READS, ((n + 1) * READS + UR - 1) / UR); ++r) read(1 - h, slot, r);
+        if (n >= UV) {
+#pragma unroll
+          for (int r = (n - UV) * UNITS / (U - UV); r < (n - UV + 1) * UNITS / (U - UV); ++r) make(1 - h, r);
+        }
+        send(n * P / U, (n + 1) * P / U);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  // two panels a way round, the second one zeros where there is none: the loop has one way out (accumulators, above)
+  const int nk = (a.nk + 1) & ~1;
+#pragma unroll
+  for (int u = 0; u < NST; ++u)
+    if (u < nk) issue(u, u, 0, P);
+  tile::wait_stages<NST - 1, P>(nk - 1);
+  tile::done_reading();
+#pragma unroll
+  for (int r = 0; r < READS; ++r) read(0, 0, r);
+#pragma unroll
+  for (int r = 0; r < UNITS; ++r) make(0, r);
+  int t = 0, s0 = 0, s1 = 1;
+  auto next = [&](int h) __attribute__((always_inline)) {
+    tile::wait_stages<NST - 2, P>(nk - 2 - t);           // panel t + 1 has arrived
+    if (t + 1 == a.nk) {                                 // (each wave clears what it sent for)
+#pragma unroll
+      for (int q = 0; q < PX; ++q) *reinterpret_cast<uint4*>(lds + s1 * SB + (wid + 4 * q) % NX * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
+    }
+    tile::done_reading();
+    const bool more = t + NST < nk;
+    step(h, s1, [&](int b, int e) __attribute__((always_inline)) { if (more) issue(t + NST, s0, b, e); });
+    s0 = s1, s1 = s1 == NST - 1 ? 0 : s1 + 1, ++t;
+  };
+  do next(0), next(1);
+  while (t < nk);
+  settle<NAMED>();
+}
+
+}  // namespace mx
+}  // namespace lumen

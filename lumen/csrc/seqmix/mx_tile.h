@@ -1,0 +1,83 @@
+// Arguments, stores and checks that the products with MXFP4 weights on tiles share (mx_loop.h).
+#pragma once
+#include "mx_loop.h"
+
+namespace lumen {
+namespace mx {
+
+struct TileArgs {
+  const void* x; long long ldx;          // rows (in MXFP4: codes)
+  const void* xs;                        // scales of rows in MXFP4
+  const void *codes, *scales;            // of the weight [N, K]
+  const void* bias;
+  void* y;
+  int M, N, K, Nx;                       // Nx: columns of dy that can be read (N up to a multiple of 8, zeros behind N)
+  int tiles_m, tiles_n, group, wide;     // wide: values a store can take, 8, 4 or 1
+};
+
+// columns n .. n + 3 (u) and n + 4 .. n + 7 (v, `two`) of row m
+template <typename T>
+__device__ __forceinline__ void put(const TileArgs& a, int m, int n, bool two, const f32x4& u, const f32x4& v) {
+  T* p = (T*)a.y + (long long)m * a.N + n;
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = u[e], r[4 + e] = v[e];
+  if (a.bias) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < (two ? 8 : 4)) r[e] += to_f32(((const T*)a.bias)[min(n + e, a.N - 1)]);
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (a.wide == 8 && two && n + 8 <= a.N) {
+      store8(p, r);
+      return;
+    }
+    if (a.wide >= 4) {
+      if (n < a.N) *reinterpret_cast<uint2*>(p) = make_uint2(pk2<T>(r[0], r[1]), pk2<T>(r[2], r[3]));
+      if (two && n + 4 < a.N) *reinterpret_cast<uint2*>(p + 4) = make_uint2(pk2<T>(r[4], r[5]), pk2<T>(r[6], r[7]));
+      return;
+    }
+  } else if (a.wide >= 4) {
+    if (n < a.N) *reinterpret_cast<float4*>(p) = make_float4(r[0], r[1], r[2], r[3]);
+    if (two && n + 4 < a.N) *reinterpret_cast<float4*>(p + 4) = make_float4(r[4], r[5], r[6], r[7]);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < (two ? 8 : 4) && n + e < a.N) p[e] = from_f32<T>(r[e]);
+}
+
+// the results of a wave, whose fragments of w stand for columns as tile::colperm says
+template <typename T, int NI, int MJ>
+__device__ __forceinline__ void put_all(const TileArgs& a, f32x4 (&acc)[NI][MJ], int m0, int n0) {
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    const int m = m0 + 16 * j + lr;
+#pragma unroll
+    for (int i = 0; i < NI; i += 2) {
+      const bool two = i + 1 < NI;
+      hold<kNamed<NI, MJ>>(acc[i][j]);
+      if (two) hold<kNamed<NI, MJ>>(acc[i + 1 < NI ? i + 1 : i][j]);
+      if (m < a.M) put<T>(a, m, n0 + 16 * i + (two ? 8 : 4) * lg, two, acc[i][j], acc[i + 1 < NI ? i + 1 : i][j]);
+    }
+  }
+}
+
+inline bool sizes_ok(int M, int N, int K) {
+  return M >= 1 && N >= 1 && M <= (1 << 24) && N <= (1 << 24) && K >= 32 && K % 32 == 0 && K <= (1 << 23);
+}
+
+// grid of BM x BN tiles over M x C results; false: too many
+inline bool plan(TileArgs& a, int C, int BM, int BN, int& grid) {
+  const long long tm = (a.M + BM - 1LL) / BM, tn = (C + BN - 1LL) / BN;
+  if (tm * tn >= (1LL << 24)) return false;
+  a.tiles_m = (int)tm, a.tiles_n = (int)tn, a.group = (int)(tm < 4 ? tm : 4);
+  grid = (int)(tm * tn);
+  return true;
+}
+
+inline int store_width(const void* y, int N, int size) { return N % 8 == 0 && (uintptr_t)y % 16 == 0 ? 8 : N % 4 == 0 && (uintptr_t)y % (4 * size) == 0 ? 4 : 1; }
+
+}  // namespace mx
+}  // namespace lumen

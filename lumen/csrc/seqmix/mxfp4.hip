@@ -7,7 +7,8 @@
 //    no logarithm, no rounding that could cross a power of two;
 //  * x / 2^e and its rounding are the hardware's scaled conversions; over all 65536 patterns of both 16-bit types and scales from the
 //    smallest to the largest they round as said above, denormals included.
-// Rows are stored padded to whole 128 values, with codes and scales of zero: the products' loads need no bounds in k.
+// A matrix lies in panels of 128 values of its rows, the last one padded with codes and scales of zero: codes [panel][row][64 bytes],
+// scales [panel][row][4 bytes].  Whatever a product reads of consecutive rows is then one run of memory, and needs no bounds in k.
 #include "mx.h"
 
 using namespace lumen;
@@ -61,25 +62,35 @@ template <typename T> __device__ __forceinline__ unsigned codes8(const uint4 (&v
   return c;
 }
 
-// four lanes a block; blockIdx.y strides over the rows
+// A workgroup: 16 rows by kPan panels, 16 lanes a row of a panel, four a block; a wave writes whole lines of four rows.
+constexpr int kPan = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, long long ldx, unsigned* __restrict__ codes,
-                                                       unsigned char* __restrict__ scales, int R, int K, int Kp) {
-  const int u = blockIdx.x * 256 + threadIdx.x, k = 8 * u;
-  if (k >= Kp) return;
-  for (int r = blockIdx.y; r < R; r += gridDim.y) {
-    uint4 v[sizeof(T) / 2];
+                                                       unsigned char* __restrict__ scales, int R, int K, int panels) {
+  const int r = blockIdx.x * 16 + (threadIdx.x >> 4), u = threadIdx.x & 15, p0 = blockIdx.y * kPan;
+  if (r >= R) return;
+  uint4 v[kPan][sizeof(T) / 2];
+#pragma unroll
+  for (int p = 0; p < kPan; ++p) {
+    const int k = 128 * (p0 + p) + 8 * u;
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      v[i] = k < K ? reinterpret_cast<const uint4*>(x + r * ldx + k)[i] : make_uint4(0, 0, 0, 0);
-    unsigned top = top8<T>(v);
+      v[p][i] = k < K ? reinterpret_cast<const uint4*>(x + r * ldx + k)[i] : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int p = 0; p < kPan; ++p) {
+    unsigned top = top8<T>(v[p]);
     top = max(top, (unsigned)__shfl_xor((int)top, 1));
     top = max(top, (unsigned)__shfl_xor((int)top, 2));
     const bool bad = top >= 0x7f800000u;
     const int s = bad ? 255 : max((int)(top >> 23) - 2, 0);
-    const unsigned c = codes8<T>(v, __uint_as_float((unsigned)s << 23));
-    codes[(long long)r * (Kp / 8) + u] = bad ? 0u : c;
-    if ((u & 3) == 0) scales[(long long)r * (Kp / 32) + (u >> 2)] = (unsigned char)s;
+    const unsigned c = codes8<T>(v[p], mx_scale(s));
+    if (p0 + p < panels) {
+      const long long row = (long long)(p0 + p) * R + r;
+      codes[row * 16 + u] = bad ? 0u : c;
+      if ((u & 3) == 0) scales[row * 4 + (u >> 2)] = (unsigned char)s;
+    }
   }
 }
 
@@ -97,43 +108,55 @@ template <typename T> __device__ __forceinline__ void values8(unsigned c, float 
 
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned* __restrict__ codes, const unsigned char* __restrict__ scales,
-                                                         T* __restrict__ y, int R, int K, int Kp) {
-  const int u = blockIdx.x * 256 + threadIdx.x;
-  if (8 * u >= K) return;
-  for (int r = blockIdx.y; r < R; r += gridDim.y) {
-    const unsigned c = codes[(long long)r * (Kp / 8) + u];
-    const unsigned s = scales[(long long)r * (Kp / 32) + (u >> 2)];
-    values8<T>(c, __uint_as_float(s << 23), y + (long long)r * K + 8 * u);
+                                                         T* __restrict__ y, int R, int K, int panels) {
+  const int r = blockIdx.x * 16 + (threadIdx.x >> 4), u = threadIdx.x & 15, p0 = blockIdx.y * kPan;
+  if (r >= R) return;
+  unsigned c[kPan], s[kPan];
+#pragma unroll
+  for (int p = 0; p < kPan; ++p) {
+    const long long row = (long long)min(p0 + p, panels - 1) * R + r;
+    c[p] = codes[row * 16 + u];
+    s[p] = scales[row * 4 + (u >> 2)];
+  }
+#pragma unroll
+  for (int p = 0; p < kPan; ++p) {
+    const int k = 128 * (p0 + p) + 8 * u;
+    if (k < K) values8<T>(c[p], mx_scale(s[p]), y + (long long)r * K + k);
   }
 }
+
+// workgroups for R rows of K values
+inline dim3 grid_of(int R, int panels) { return dim3((R + 15) / 16, (panels + kPan - 1) / kPan); }
 
 }  // namespace
 
 extern "C" {
 
-// codes [R, Kp / 2], scales [R, Kp / 32] of x [R, K] at ldx; K % 32 == 0, Kp: K rounded up to 128, rows of x at 16-byte addresses
+// codes [panels, R, 64], scales [panels, R, 4] of x [R, K] at ldx; K % 32 == 0, panels of 128 values, rows of x at 16-byte addresses
 hipError_t sm_mx_quantize(int dt, const void* x, long long ldx, void* codes, void* scales, int R, int K, hipStream_t st) {
-  const int Kp = (K + 127) / 128 * 128;
-  if (R < 1 || K < 32 || K % 32 || K > (1 << 23) || ldx < K || ldx % (dt == kF32 ? 4 : 8) || (uintptr_t)x % 16 || (uintptr_t)codes % 16 ||
-      (uintptr_t)scales % 4 || (dt != kF16 && dt != kBF16 && dt != kF32))
+  const int P = (K + 127) / 128;
+  if (R < 1 || R > (1 << 24) || K < 32 || K % 32 || K > (1 << 23) || ldx < K || ldx % (dt == kF32 ? 4 : 8) || (uintptr_t)x % 16 ||
+      (uintptr_t)codes % 16 || (uintptr_t)scales % 4 || (dt != kF16 && dt != kBF16 && dt != kF32))
     return hipErrorInvalidValue;
-  const dim3 grid((Kp / 8 + 255) / 256, R < 65535 ? R : 65535);
-  if (dt == kF32) quantize_kernel<float><<<grid, 256, 0, st>>>((const float*)x, ldx, (unsigned*)codes, (unsigned char*)scales, R, K, Kp);
-  else if (dt == kBF16) quantize_kernel<bf16><<<grid, 256, 0, st>>>((const bf16*)x, ldx, (unsigned*)codes, (unsigned char*)scales, R, K, Kp);
-  else quantize_kernel<fp16><<<grid, 256, 0, st>>>((const fp16*)x, ldx, (unsigned*)codes, (unsigned char*)scales, R, K, Kp);
+  unsigned* c = (unsigned*)codes;
+  unsigned char* s = (unsigned char*)scales;
+  if (dt == kF32) quantize_kernel<float><<<grid_of(R, P), 256, 0, st>>>((const float*)x, ldx, c, s, R, K, P);
+  else if (dt == kBF16) quantize_kernel<bf16><<<grid_of(R, P), 256, 0, st>>>((const bf16*)x, ldx, c, s, R, K, P);
+  else quantize_kernel<fp16><<<grid_of(R, P), 256, 0, st>>>((const fp16*)x, ldx, c, s, R, K, P);
   return hipGetLastError();
 }
 
 // y [R, K] of such codes and scales
 hipError_t sm_mx_dequantize(int dt, const void* codes, const void* scales, void* y, int R, int K, hipStream_t st) {
-  const int Kp = (K + 127) / 128 * 128;
-  if (R < 1 || K < 32 || K % 32 || K > (1 << 23) || (uintptr_t)y % 16 || (uintptr_t)codes % 16 || (uintptr_t)scales % 4 ||
+  const int P = (K + 127) / 128;
+  if (R < 1 || R > (1 << 24) || K < 32 || K % 32 || K > (1 << 23) || (uintptr_t)y % 16 || (uintptr_t)codes % 16 || (uintptr_t)scales % 4 ||
       (dt != kF16 && dt != kBF16 && dt != kF32))
     return hipErrorInvalidValue;
-  const dim3 grid((K / 8 + 255) / 256, R < 65535 ? R : 65535);
-  if (dt == kF32) dequantize_kernel<float><<<grid, 256, 0, st>>>((const unsigned*)codes, (const unsigned char*)scales, (float*)y, R, K, Kp);
-  else if (dt == kBF16) dequantize_kernel<bf16><<<grid, 256, 0, st>>>((const unsigned*)codes, (const unsigned char*)scales, (bf16*)y, R, K, Kp);
-  else dequantize_kernel<fp16><<<grid, 256, 0, st>>>((const unsigned*)codes, (const unsigned char*)scales, (fp16*)y, R, K, Kp);
+  const unsigned* c = (const unsigned*)codes;
+  const unsigned char* s = (const unsigned char*)scales;
+  if (dt == kF32) dequantize_kernel<float><<<grid_of(R, P), 256, 0, st>>>(c, s, (float*)y, R, K, P);
+  else if (dt == kBF16) dequantize_kernel<bf16><<<grid_of(R, P), 256, 0, st>>>(c, s, (bf16*)y, R, K, P);
+  else dequantize_kernel<fp16><<<grid_of(R, P), 256, 0, st>>>(c, s, (fp16*)y, R, K, P);
   return hipGetLastError();
 }
 

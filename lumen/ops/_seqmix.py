@@ -88,9 +88,9 @@ SIGNATURES = {
     "sm_thin_act": "iplppp" "iiiiiiiii" "ffff",
     "sm_mx_quantize": "iplppii",
     "sm_mx_dequantize": "ipppii",
-    "sm_mx_linear": "iplppppiii",
-    "sm_mx_grad": "iplpppiii",
-    "sm_mx_matmul": "ippppppiii",
+    "sm_mx_linear": "iplppppiiiii",
+    "sm_mx_grad": "iplpppiiiii",
+    "sm_mx_matmul": "ippppppiiiii",
 }
 
 

@@ -14,23 +14,26 @@ weight holds no gradient: it is the frozen base of adapters, or served.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
+import torch.nn.functional as F
 
 from ._seqmix import DT, call, use_seqmix
 
 BLOCK = 32                # values that share a scale
-PAD = 128                 # rows are stored in whole 128 values: the products' loads need no bounds along k
-MAX_K = 1 << 23
+PANEL = 128               # values of a row that lie together (csrc/seqmix/mxfp4.hip)
+MAX_K, MAX_ROWS = 1 << 23, 1 << 24
 HALF = (torch.bfloat16, torch.float16)
 
 
 class MXFP4:
     """A matrix [rows, K] in MXFP4: ``codes`` uint8 [rows, K / 2], ``scales`` uint8 [rows, K / 32].
 
-    Built from such tensors (of another program's checkpoint, say) or by ``mxfp4_quantize``.  Rows whose K is no multiple
-    of 128 are copied into rows padded with zeros; the others are held as they are."""
+    Built from such tensors (of another program's checkpoint, say) or by ``mxfp4_quantize``.  It holds them in panels of 128
+    values, [panel, row, 64] and [panel, row, 4] bytes, zeros behind a row's end, as the kernels read them; ``codes`` and
+    ``scales`` give copies in rows."""
 
     __slots__ = ("shape", "_codes", "_scales")
 
@@ -40,21 +43,21 @@ class MXFP4:
         R, K = codes.shape[0], 2 * codes.shape[1]
         if scales.shape[0] != R or scales.shape[1] * BLOCK != K:
             raise ValueError(f"MXFP4: scales {list(scales.shape)} do not fit codes {list(codes.shape)}")
-        if not 0 < K <= MAX_K:
-            raise ValueError(f"MXFP4: rows of {K} values (32 to {MAX_K})")
+        if not 0 < K <= MAX_K or R > MAX_ROWS:
+            raise ValueError(f"MXFP4: {R} rows of {K} values (at most {MAX_ROWS}, and 32 to {MAX_K})")
         if codes.device != scales.device:
             raise ValueError(f"MXFP4: codes on {codes.device}, scales on {scales.device}")
         self.shape = (R, K)
-        self._codes = _padded(codes, PAD // 2)
-        self._scales = _padded(scales, PAD // BLOCK)
+        self._codes = _panels(codes.detach(), PANEL // 2)
+        self._scales = _panels(scales.detach(), PANEL // BLOCK)
 
     @property
     def codes(self) -> torch.Tensor:
-        return self._codes[:, :self.shape[1] // 2]
+        return _rows_of(self._codes)[:, :self.shape[1] // 2]
 
     @property
     def scales(self) -> torch.Tensor:
-        return self._scales[:, :self.shape[1] // BLOCK]
+        return _rows_of(self._scales)[:, :self.shape[1] // BLOCK]
 
     @property
     def device(self) -> torch.device:
@@ -65,7 +68,7 @@ class MXFP4:
         return self._codes.numel() + self._scales.numel()
 
     def to(self, device) -> "MXFP4":
-        return self if self._codes.device == torch.device(device) else MXFP4(self.codes.to(device), self.scales.to(device))
+        return _of(self._codes.to(device), self._scales.to(device), self.shape[1])
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         return mxfp4_dequantize(self, dtype)
@@ -74,20 +77,27 @@ class MXFP4:
         return f"MXFP4({self.shape[0]} x {self.shape[1]}, {self.device})"
 
 
-def _padded(t: torch.Tensor, unit: int) -> torch.Tensor:
-    """``t`` in contiguous, aligned rows of a multiple of ``unit`` bytes, zeros behind its own."""
-    t = t.detach()
-    n = -(-t.shape[1] // unit) * unit
-    if n == t.shape[1] and t.is_contiguous() and t.data_ptr() % 16 == 0:
-        return t
-    out = torch.zeros(t.shape[0], n, dtype=t.dtype, device=t.device)
-    out[:, :t.shape[1]] = t
+def _panels(t: torch.Tensor, unit: int) -> torch.Tensor:
+    """[rows, n] bytes -> [panels, rows, unit], zeros behind a row's last one."""
+    R, n = t.shape
+    P = -(-n // unit)
+    out = torch.zeros(P, R, unit, dtype=t.dtype, device=t.device)
+    whole = n // unit
+    out[:whole].copy_(t[:, :whole * unit].reshape(R, whole, unit).transpose(0, 1))
+    if whole < P:
+        out[whole, :, :n - whole * unit].copy_(t[:, whole * unit:])
     return out
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """[panels, rows, unit] bytes -> [rows, panels * unit], a copy."""
+    P, R, unit = t.shape
+    return t.transpose(0, 1).reshape(R, P * unit)
 
 
 def _of(codes: torch.Tensor, scales: torch.Tensor, K: int) -> MXFP4:
     q = MXFP4.__new__(MXFP4)
-    q.shape, q._codes, q._scales = (codes.shape[0], K), codes, scales
+    q.shape, q._codes, q._scales = (codes.shape[1], K), codes, scales
     return q
 
 
@@ -115,14 +125,14 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4:
     if x.dim() != 2 or x.dtype not in DT:
         raise ValueError("mxfp4_quantize: a matrix [rows, K] of fp32, bf16 or fp16")
     R, K = x.shape
-    if K % BLOCK or not 0 < K <= MAX_K:
-        raise ValueError(f"mxfp4_quantize: rows of {K} values (a multiple of {BLOCK}, at most {MAX_K})")
+    if K % BLOCK or not 0 < K <= MAX_K or R > MAX_ROWS:
+        raise ValueError(f"mxfp4_quantize: {R} rows of {K} values (at most {MAX_ROWS}; a multiple of {BLOCK}, at most {MAX_K})")
     x = x.detach()
     if not use_seqmix(x):
         return MXFP4(*_encode(x))
-    Kp = -(-K // PAD) * PAD
-    codes = torch.empty(R, Kp // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(R, Kp // BLOCK, dtype=torch.uint8, device=x.device)
+    P = -(-K // PANEL)
+    codes = torch.empty(P, R, PANEL // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(P, R, PANEL // BLOCK, dtype=torch.uint8, device=x.device)
     if R:
         with _on(x.device):
             x = _rows(x, 16 // x.element_size())
@@ -178,6 +188,32 @@ def _decode(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return (v * _power(scales).unsqueeze(-1)).reshape(R, n * BLOCK)
 
 
+def _best(M: int, N: int, tiles, cost) -> tuple:
+    """The tile of ``tiles`` (rows, columns, ...) whose rounds of 256 workgroups take the least time, ``cost`` a stage."""
+    return min(tiles, key=lambda t: -(-(-(-M // t[0]) * -(-N // t[1])) // 256) * cost(t))
+
+
+_LINEAR = [(32 * mj, 32 * ni, mj, ni) for mj, ni in ((8, 8), (8, 6), (8, 4), (8, 2), (4, 8), (4, 4), (4, 2), (2, 8), (2, 4), (2, 2), (2, 1), (1, 8),
+                                                    (1, 4), (1, 2), (1, 1))]
+_MATMUL = [t for t in _LINEAR if t[2:] not in ((8, 6), (8, 2))]
+_GRAD = [(64 * mj // wn, 128 * wn, mj, wn) for mj, wn in ((8, 2), (4, 2), (2, 2), (1, 2), (4, 1), (2, 1), (1, 1))]
+
+
+@functools.lru_cache(4096)
+def _linear_tile(M: int, N: int) -> tuple:
+    return _best(M, N, _LINEAR, lambda t: max(t[0] * t[1] / 32, (t[0] * 128 + t[1] * 36) / 48) + 200)[2:]
+
+
+@functools.lru_cache(4096)
+def _grad_tile(M: int, K: int) -> tuple:
+    return _best(M, K, _GRAD, lambda t: max(t[0] * t[1] / 32, (t[0] * 128 + t[1] * 36) / 48) + 400)[2:]
+
+
+@functools.lru_cache(4096)
+def _matmul_tile(M: int, N: int) -> tuple:
+    return _best(M, N, _MATMUL, lambda t: max(t[0] * t[1] / 64, (t[0] + t[1]) * 68 / 48) + 200)[2:]
+
+
 # ---- products ---------------------------------------------------------------------------------------
 def _check(name: str, K: int, device, w, bias: Optional[torch.Tensor], dtype: torch.dtype) -> None:
     if not isinstance(w, MXFP4):
@@ -200,7 +236,7 @@ def _linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor]) -> torch.Te
     if M and N:
         with _on(x.device):
             x = _rows(x)
-            call("sm_mx_linear", DT[x.dtype], x, _ld(x), w._codes, w._scales, None if bias is None else bias.contiguous(), y, M, N, K)
+            call("sm_mx_linear", DT[x.dtype], x, _ld(x), w._codes, w._scales, None if bias is None else bias.contiguous(), y, M, N, K, *_linear_tile(M, N))
     return y
 
 
@@ -213,8 +249,8 @@ def _input_grad(dy: torch.Tensor, w: MXFP4) -> torch.Tensor:
         return torch.zeros(M, K, dtype=dy.dtype, device=dy.device)
     dx = torch.empty(M, K, dtype=dy.dtype, device=dy.device)
     with _on(dy.device):
-        dy = _rows(dy)
-        call("sm_mx_grad", DT[dy.dtype], dy, _ld(dy), w._codes, w._scales, dx, M, N, K)
+        dy = F.pad(dy, (0, -N % 8)) if N % 8 else _rows(dy)          # (rows at 16-byte addresses, zeros behind them)
+        call("sm_mx_grad", DT[dy.dtype], dy, _ld(dy), w._codes, w._scales, dx, M, N, K, *_grad_tile(M, K))
     return dx
 
 
@@ -268,5 +304,5 @@ def mxfp4_matmul(a: MXFP4, b: MXFP4, bias: Optional[torch.Tensor] = None, out_dt
     if M and N:
         with _on(a.device):
             call("sm_mx_matmul", DT[out_dtype], a._codes, a._scales, b._codes, b._scales,
-                 None if bias is None else bias.contiguous(), y, M, N, K)
+                 None if bias is None else bias.contiguous(), y, M, N, K, *_matmul_tile(M, N))
     return y
