@@ -53,7 +53,7 @@ hipError_t sm_mx_linear(int dt, const void* x, long long ldx, const void* codes,
     if (dt == kBF16) linear_kernel<bf16, NI, MJ, 2><<<grid, 256, 0, st>>>(a);          \
     else linear_kernel<fp16, NI, MJ, 2><<<grid, 256, 0, st>>>(a);                      \
     break;
-    GO(1, 1) GO(1, 2) GO(1, 4) GO(1, 8) GO(2, 1) GO(2, 2) GO(2, 4) GO(2, 8) GO(4, 2) GO(4, 4) GO(4, 8) GO(8, 2) GO(8, 4) GO(8, 6) GO(8, 8)
+    GO(8, 4) GO(8, 6) GO(8, 8)
 #undef GO
     default: return hipErrorInvalidValue;
   }

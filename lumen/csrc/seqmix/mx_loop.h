@@ -37,6 +37,16 @@ __device__ __forceinline__ unsigned lds_addr(const char* p) {
   return (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p);
 }
 
+// f(0) ... f(N - 1), each with its number as a constant (a loop's bounds and choices by it cost the unroller too much)
+template <int N> struct Int { static constexpr int value = N; };
+template <int A, int B, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (A < B) {
+    f(Int<A>{});
+    each<A + 1, B>(f);
+  }
+}
+
 // two 16-bit values of byte W of eight codes, in the place where it is written: a product may follow two instructions later
 template <typename T, int W>
 __device__ __forceinline__ unsigned pair(unsigned c, float scale) {
@@ -57,6 +67,16 @@ __device__ __forceinline__ unsigned pair(unsigned c, float scale) {
 
 // what the vector unit wrote is there for the matrix core
 __device__ __forceinline__ void ready() { asm volatile("s_nop 1" ::: "memory"); }
+
+// values of byte W of two rows' codes c0 and c1, regrouped by column: x the pair (row 0, row 1) of the even column, y of the odd one
+template <typename T, int W>
+__device__ __forceinline__ uint2 columns(unsigned c0, unsigned c1, float s0, float s1) {
+  const unsigned p = pair<T, W>(c0, s0), q = pair<T, W>(c1, s1);
+  unsigned even, odd;
+  asm volatile("v_perm_b32 %0, %1, %2, %3" : "=v"(even) : "v"(q), "v"(p), "s"(0x05040100u));
+  asm volatile("v_perm_b32 %0, %1, %2, %3" : "=v"(odd) : "v"(q), "v"(p), "s"(0x07060302u));
+  return make_uint2(even, odd);
+}
 
 // ---- 16-bit rows against 4-bit weights -------------------------------------------------------------
 //
@@ -168,44 +188,31 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
   };
   // unit n of the making of half h's fragments of w; t: their stage
   constexpr int UNITS = GRAD ? 16 : 4 * NI;
-  auto make = [&](int h, int t, int n) __attribute__((always_inline)) {
-    const int w = n & 3, u = n >> 2;
+  auto make = [&](int h, int t, auto num) __attribute__((always_inline)) {
+    constexpr int n = decltype(num)::value, w = n & 3, u = n >> 2;
     if constexpr (GRAD) {                                // rows 2 u and 2 u + 1, columns 2 w and 2 w + 1
-      if (w == 0) fs[0] = mx_scale(sc[2 * u]), fs[1] = mx_scale(sc[2 * u + 1]);
-      unsigned p, q;
-      if (w == 0) p = pair<T, 0>(raw[2 * u], fs[0]), q = pair<T, 0>(raw[2 * u + 1], fs[1]);
-      else if (w == 1) p = pair<T, 1>(raw[2 * u], fs[0]), q = pair<T, 1>(raw[2 * u + 1], fs[1]);
-      else if (w == 2) p = pair<T, 2>(raw[2 * u], fs[0]), q = pair<T, 2>(raw[2 * u + 1], fs[1]);
-      else p = pair<T, 3>(raw[2 * u], fs[0]), q = pair<T, 3>(raw[2 * u + 1], fs[1]);
-      asm volatile("v_perm_b32 %0, %1, %2, %3" : "=v"(fw[h][2 * w][u]) : "v"(q), "v"(p), "s"(0x05040100u));
-      asm volatile("v_perm_b32 %0, %1, %2, %3" : "=v"(fw[h][2 * w + 1][u]) : "v"(q), "v"(p), "s"(0x07060302u));
+      if constexpr (w == 0) fs[0] = mx_scale(sc[2 * u]), fs[1] = mx_scale(sc[2 * u + 1]);
+      const uint2 v = columns<T, w>(raw[2 * u], raw[2 * u + 1], fs[0], fs[1]);
+      fw[h][2 * w][u] = v.x, fw[h][2 * w + 1][u] = v.y;
     } else {
-      if (w == 0) fs[0] = mx_scale((sc[u] >> (16 * (t & 1) + 8 * h)) & 255u);
-      if (w == 0) fw[h][u][0] = pair<T, 0>(raw[u], fs[0]);
-      else if (w == 1) fw[h][u][1] = pair<T, 1>(raw[u], fs[0]);
-      else if (w == 2) fw[h][u][2] = pair<T, 2>(raw[u], fs[0]);
-      else fw[h][u][3] = pair<T, 3>(raw[u], fs[0]);
+      if constexpr (w == 0) fs[0] = mx_scale((sc[u] >> (16 * (t & 1) + 8 * h)) & 255u);
+      fw[h][u][w] = pair<T, w>(raw[u], fs[0]);
     }
   };
   // the products of half h, between them reads and making of the other half, of stage t2 in `slot`, and send(a, b): pieces a .. b - 1
   auto half = [&](int h, int t2, int slot, auto&& send) __attribute__((always_inline)) {
-    constexpr int U = NI * MJ, UR = (U * 3 + 7) / 8, UV = U / 4;         // reads in products 0 .. UR - 1, making from UV on
+    constexpr int U = NI * MJ, UR = (U * 3 + 7) / 8, UV = U < 48 ? U / 2 : U / 4;        // reads in products 0 .. UR - 1, making from UV on
     ready();
-#pragma unroll
-    for (int j = 0; j < MJ; ++j)
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int n = j * NI + i;
-        mfma<T, NAMED>(acc[i][j], make_uint4(fw[h][i][0], fw[h][i][1], fw[h][i][2], fw[h][i][3]), fx[h][j]);
-#pragma unroll
-        for (int r = min(READS, (n * READS + UR - 1) / UR); r < min(READS, ((n + 1) * READS + UR - 1) / UR); ++r) read(1 - h, slot, r);
-        if (n >= UV) {
-#pragma unroll
-          for (int r = (n - UV) * UNITS / (U - UV); r < (n - UV + 1) * UNITS / (U - UV); ++r) make(1 - h, t2, r);
-        }
-        send(n * P / U, (n + 1) * P / U);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    each<0, U>([&](auto num) __attribute__((always_inline)) {
+      constexpr int n = decltype(num)::value, i = n % NI, j = n / NI;
+      mfma<T, NAMED>(acc[i][j], make_uint4(fw[h][i][0], fw[h][i][1], fw[h][i][2], fw[h][i][3]), fx[h][j]);
+      constexpr int r0 = (n * READS + UR - 1) / UR, r1 = ((n + 1) * READS + UR - 1) / UR;
+      each<(r0 < READS ? r0 : READS), (r1 < READS ? r1 : READS)>([&](auto r) __attribute__((always_inline)) { read(1 - h, slot, r.value); });
+      if constexpr (n >= UV)
+        each<(n - UV) * UNITS / (U - UV), (n - UV + 1) * UNITS / (U - UV)>([&](auto r) __attribute__((always_inline)) { make(1 - h, t2, r); });
+      send(n * P / U, (n + 1) * P / U);
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
   const auto none = [](int, int) __attribute__((always_inline)) {};
   const int nk = a.nk;
@@ -218,8 +225,7 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
   tile::done_reading();
 #pragma unroll
   for (int r = 0; r < READS; ++r) read(0, 0, r);
-#pragma unroll
-  for (int r = 0; r < UNITS; ++r) make(0, 0, r);
+  each<0, UNITS>([&](auto r) __attribute__((always_inline)) { make(0, 0, r); });
   for (int t = 0, s0 = 0, s1 = 1;;) {                    // slots of stages t and t + 1
     half(0, t, s0, none);
     tile::wait_stages<NST - 2, P>(nk - 2 - t);           // stage t + 1 has arrived
@@ -308,21 +314,16 @@ __device__ __forceinline__ void products4(char* lds, const Walk4& a, const unsig
   auto step = [&](int h, int slot, auto&& send) __attribute__((always_inline)) {
     constexpr int U = NI * MJ, UR = (U * 5 + 7) / 8, UV = U / 2;
     ready();
-#pragma unroll
-    for (int j = 0; j < MJ; ++j)
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int n = j * NI + i;
-        mfma4<NAMED>(acc[i][j], fw[h][i], fx[h][j], sw[h][i], sx[h][j]);
-#pragma unroll
-        for (int r = min(READS, (n * READS + UR - 1) / UR); r < min(READS, ((n + 1) * READS + UR - 1) / UR); ++r) read(1 - h, slot, r);
-        if (n >= UV) {
-#pragma unroll
-          for (int r = (n - UV) * UNITS / (U - UV); r < (n - UV + 1) * UNITS / (U - UV); ++r) make(1 - h, r);
-        }
-        send(n * P / U, (n + 1) * P / U);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    each<0, U>([&](auto num) __attribute__((always_inline)) {
+      constexpr int n = decltype(num)::value, i = n % NI, j = n / NI;
+      mfma4<NAMED>(acc[i][j], fw[h][i], fx[h][j], sw[h][i], sx[h][j]);
+      constexpr int r0 = (n * READS + UR - 1) / UR, r1 = ((n + 1) * READS + UR - 1) / UR;
+      each<(r0 < READS ? r0 : READS), (r1 < READS ? r1 : READS)>([&](auto r) __attribute__((always_inline)) { read(1 - h, slot, r.value); });
+      if constexpr (n >= UV)
+        each<(n - UV) * UNITS / (U - UV), (n - UV + 1) * UNITS / (U - UV)>([&](auto r) __attribute__((always_inline)) { make(1 - h, r.value); });
+      send(n * P / U, (n + 1) * P / U);
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
   // two panels a way round, the second one zeros where there is none: the loop has one way out (accumulators, above)
   const int nk = (a.nk + 1) & ~1;

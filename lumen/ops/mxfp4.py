@@ -20,22 +20,24 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
-from ._seqmix import DT, call, use_seqmix
+from . import _seqmix
+from ._seqmix import DT, use_seqmix
 
 BLOCK = 32                # values that share a scale
 PANEL = 128               # values of a row that lie together (csrc/seqmix/mxfp4.hip)
 MAX_K, MAX_ROWS = 1 << 23, 1 << 24
+MAX_LD = 1 << 22          # values from row to row that the products take
 HALF = (torch.bfloat16, torch.float16)
 
 
 class MXFP4:
     """A matrix [rows, K] in MXFP4: ``codes`` uint8 [rows, K / 2], ``scales`` uint8 [rows, K / 32].
 
-    Built from such tensors (of another program's checkpoint, say) or by ``mxfp4_quantize``.  It holds them in panels of 128
-    values, [panel, row, 64] and [panel, row, 4] bytes, zeros behind a row's end, as the kernels read them; ``codes`` and
-    ``scales`` give copies in rows."""
+    Built from such tensors (of another program's checkpoint, say) or by ``mxfp4_quantize``.  It holds them as the kernels read
+    them, in panels of 128 values of all rows: [panel, row, 64] bytes of codes, then [panel, row, 4] of scales, zeros behind a
+    row's end; ``codes`` and ``scales`` give copies in rows."""
 
-    __slots__ = ("shape", "_codes", "_scales")
+    __slots__ = ("shape", "data")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
@@ -48,8 +50,21 @@ class MXFP4:
         if codes.device != scales.device:
             raise ValueError(f"MXFP4: codes on {codes.device}, scales on {scales.device}")
         self.shape = (R, K)
-        self._codes = _panels(codes.detach(), PANEL // 2)
-        self._scales = _panels(scales.detach(), PANEL // BLOCK)
+        self.data = torch.zeros(_nbytes(R, K), dtype=torch.uint8, device=codes.device)
+        _fill(self._codes, codes.detach())
+        _fill(self._scales, scales.detach())
+
+    @property
+    def _codes(self) -> torch.Tensor:
+        R, K = self.shape
+        P = -(-K // PANEL)
+        return self.data[:P * R * 64].view(P, R, 64)
+
+    @property
+    def _scales(self) -> torch.Tensor:
+        R, K = self.shape
+        P = -(-K // PANEL)
+        return self.data[P * R * 64:].view(P, R, 4)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -61,14 +76,14 @@ class MXFP4:
 
     @property
     def device(self) -> torch.device:
-        return self._codes.device
+        return self.data.device
 
     @property
     def nbytes(self) -> int:
-        return self._codes.numel() + self._scales.numel()
+        return self.data.numel()
 
     def to(self, device) -> "MXFP4":
-        return _of(self._codes.to(device), self._scales.to(device), self.shape[1])
+        return _of(self.data.to(device), self.shape)
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         return mxfp4_dequantize(self, dtype)
@@ -77,16 +92,17 @@ class MXFP4:
         return f"MXFP4({self.shape[0]} x {self.shape[1]}, {self.device})"
 
 
-def _panels(t: torch.Tensor, unit: int) -> torch.Tensor:
-    """[rows, n] bytes -> [panels, rows, unit], zeros behind a row's last one."""
-    R, n = t.shape
-    P = -(-n // unit)
-    out = torch.zeros(P, R, unit, dtype=t.dtype, device=t.device)
+def _nbytes(R: int, K: int) -> int:
+    return -(-K // PANEL) * R * 68
+
+
+def _fill(panels: torch.Tensor, t: torch.Tensor) -> None:
+    """[rows, n] bytes into [panels, rows, unit] ones."""
+    unit, n = panels.shape[2], t.shape[1]
     whole = n // unit
-    out[:whole].copy_(t[:, :whole * unit].reshape(R, whole, unit).transpose(0, 1))
-    if whole < P:
-        out[whole, :, :n - whole * unit].copy_(t[:, whole * unit:])
-    return out
+    panels[:whole].copy_(t[:, :whole * unit].reshape(t.shape[0], whole, unit).transpose(0, 1))
+    if n % unit:
+        panels[whole, :, :n % unit].copy_(t[:, whole * unit:])
 
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
@@ -95,28 +111,50 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
     return t.transpose(0, 1).reshape(R, P * unit)
 
 
-def _of(codes: torch.Tensor, scales: torch.Tensor, K: int) -> MXFP4:
+def _of(data: torch.Tensor, shape: tuple) -> MXFP4:
     q = MXFP4.__new__(MXFP4)
-    q.shape, q._codes, q._scales = (codes.shape[1], K), codes, scales
+    q.data, q.shape = data, shape
     return q
 
 
-def _rows(x: torch.Tensor, unit: int = 8) -> torch.Tensor:
-    """``x`` [rows, K] itself where its rows are contiguous and at 16-byte addresses, else a copy."""
+def _addresses(q: MXFP4) -> tuple:
+    """Of its codes and scales."""
+    R, K = q.shape
+    p = q.data.data_ptr()
+    return p, p + -(-K // PANEL) * R * 64
+
+
+def _rows(x: torch.Tensor, unit: int = 8) -> tuple:
+    """(``x`` [rows, K] itself where its rows are contiguous and at 16-byte addresses, else a copy; its address; values from row to row)."""
+    R, K = x.shape
     if x.is_neg():
         x = x.resolve_neg()
-    if x.stride(1) == 1 and x.data_ptr() % 16 == 0 and (x.shape[0] < 2 or x.stride(0) % unit == 0 and x.stride(0) >= x.shape[1]):
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+    ld, one = x.stride()
+    if R == 1:
+        ld = -(-K // unit) * unit
+    p = x.data_ptr()
+    if (one != 1 and K > 1) or p % 16 or ld % unit or not K <= ld <= MAX_LD:
+        x = x.clone(memory_format=torch.contiguous_format)
+        p, ld = x.data_ptr(), K
+    return x, p, ld
 
 
-def _ld(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+_fns: dict = {}
 
 
-def _on(device: torch.device):
-    """The device's context (its current stream) where it is not the current one already."""
-    return torch.cuda.device(device)
+def _launch(name: str, device: torch.device, *args) -> None:
+    """The library's ``name`` on the current stream of ``device``, which becomes the current device for it."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_seqmix._load(), name)
+    i = device.index
+    if i == torch._C._cuda_getDevice():            # (nearly always: as little host time as can be)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        raise RuntimeError(f"{name}: HIP error {rc}")
 
 
 # ---- the format -------------------------------------------------------------------------------------
@@ -127,17 +165,14 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4:
     R, K = x.shape
     if K % BLOCK or not 0 < K <= MAX_K or R > MAX_ROWS:
         raise ValueError(f"mxfp4_quantize: {R} rows of {K} values (at most {MAX_ROWS}; a multiple of {BLOCK}, at most {MAX_K})")
-    x = x.detach()
     if not use_seqmix(x):
-        return MXFP4(*_encode(x))
-    P = -(-K // PANEL)
-    codes = torch.empty(P, R, PANEL // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(P, R, PANEL // BLOCK, dtype=torch.uint8, device=x.device)
+        return MXFP4(*_encode(x.detach()))
+    dev, dt = x.device, DT[x.dtype]
+    q = _of(torch.empty(_nbytes(R, K), dtype=torch.uint8, device=dev), (R, K))
     if R:
-        with _on(x.device):
-            x = _rows(x, 16 // x.element_size())
-            call("sm_mx_quantize", DT[x.dtype], x, _ld(x), codes, scales, R, K)
-    return _of(codes, scales, K)
+        x, p, ld = _rows(x.detach() if x.requires_grad else x, 8 if dt else 4)
+        _launch("sm_mx_quantize", dev, dt, p, ld, *_addresses(q), R, K)
+    return q
 
 
 def mxfp4_dequantize(q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -145,13 +180,12 @@ def mxfp4_dequantize(q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
     its largest number).  What lies beyond ``dtype``'s largest number becomes infinite."""
     if dtype not in DT:
         raise ValueError("mxfp4_dequantize: fp32, bf16 or fp16")
-    R, K = q.shape
-    if not use_seqmix(q._codes):
+    if not use_seqmix(q.data):
         return _decode(q.codes, q.scales).to(dtype)
-    y = torch.empty(R, K, dtype=dtype, device=q.device)
+    R, K = q.shape
+    y = torch.empty(R, K, dtype=dtype, device=q.data.device)
     if R:
-        with _on(q.device):
-            call("sm_mx_dequantize", DT[dtype], q._codes, q._scales, y, R, K)
+        _launch("sm_mx_dequantize", y.device, DT[dtype], *_addresses(q), y.data_ptr(), R, K)
     return y
 
 
@@ -188,55 +222,75 @@ def _decode(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return (v * _power(scales).unsqueeze(-1)).reshape(R, n * BLOCK)
 
 
-def _best(M: int, N: int, tiles, cost) -> tuple:
-    """The tile of ``tiles`` (rows, columns, ...) whose rounds of 256 workgroups take the least time, ``cost`` a stage."""
-    return min(tiles, key=lambda t: -(-(-(-M // t[0]) * -(-N // t[1])) // 256) * cost(t))
+# What a round of 256 workgroups takes, us (bf16, weights from HBM): (a + b rt) a stage of 64 k and (f + g rt) beside them on the
+# few-row kernel's xr x 16 rt results, c and e on tiles of 32 mj x 32 ni.  Measured with one round: 64 x 16 results at K = 4096 / 11008 11.4 /
+# 26, 64 x 128 23 / 51, 32 x 16 7.9 / 16, 16 x 16 5.8 / 10.8, 4 x 16 4.8 / 8.3; 256 x 128 64 / 171, 256 x 256 107 / 267.  Up to some 500
+# rows the few-row kernel's small results fill the chip (509 x 4096 x 4096 33 -> 23 us), beyond them tiles read x fewer times.
+_ROWS = [(xr, 16 * rt, (0, xr, rt), a + b * rt, f + g * rt)
+         for xr, a, b, f, g in ((4, 0.026, 0.0062, 2.5, 0.2), (16, 0.035, 0.0105, 2.8, 0.1), (32, 0.063, 0.0155, 2.8, 0.15), (64, 0.118, 0.0187, 2.2, 0.43))
+         for rt in (1, 2, 3, 4, 6, 8)]
+_TILES = [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.95, 6.0), (6, 1.15, 7.0), (8, 1.48, 12.0))]
 
 
-_LINEAR = [(32 * mj, 32 * ni, mj, ni) for mj, ni in ((8, 8), (8, 6), (8, 4), (8, 2), (4, 8), (4, 4), (4, 2), (2, 8), (2, 4), (2, 2), (2, 1), (1, 8),
-                                                    (1, 4), (1, 2), (1, 1))]
-_MATMUL = [t for t in _LINEAR if t[2:] not in ((8, 6), (8, 2))]
-_GRAD = [(64 * mj // wn, 128 * wn, mj, wn) for mj, wn in ((8, 2), (4, 2), (2, 2), (1, 2), (4, 1), (2, 1), (1, 1))]
-
-
-@functools.lru_cache(4096)
-def _linear_tile(M: int, N: int) -> tuple:
-    return _best(M, N, _LINEAR, lambda t: max(t[0] * t[1] / 32, (t[0] * 128 + t[1] * 36) / 48) + 200)[2:]
-
-
-@functools.lru_cache(4096)
-def _grad_tile(M: int, K: int) -> tuple:
-    return _best(M, K, _GRAD, lambda t: max(t[0] * t[1] / 32, (t[0] * 128 + t[1] * 36) / 48) + 400)[2:]
+def _best(M: int, N: int, K: int, forms) -> tuple:
+    """The form of ``forms`` (rows, columns, form, us a stage, us beside) whose rounds of workgroups take the least time."""
+    return min(forms, key=lambda f: -(-(-(-M // f[0]) * -(-N // f[1])) // 256) * (f[3] * (K / 64) + f[4]))[2]
 
 
 @functools.lru_cache(4096)
-def _matmul_tile(M: int, N: int) -> tuple:
-    return _best(M, N, _MATMUL, lambda t: max(t[0] * t[1] / 64, (t[0] + t[1]) * 68 / 48) + 200)[2:]
+def _linear_form(M: int, N: int, K: int) -> tuple:
+    """(0, rows, 16 columns) of the few-row kernel or (1, mj, ni) of the tiles for x [M, K] against a weight [N, K]."""
+    return _best(M, N, K, _ROWS + _TILES if M > 64 else [f for f in _ROWS if f[0] >= min(M, 64)])
+
+
+_MATMUL = [(32 * mj, 32 * ni, (mj, ni), max(mj * ni * 8, (mj + ni) * 23) + 100, 0)
+           for mj, ni in ((8, 8), (8, 4), (4, 8), (4, 4), (4, 2), (2, 8), (2, 4), (2, 2), (2, 1), (1, 8), (1, 4), (1, 2), (1, 1))]
+# the gradient likewise, a stage 64 of the weight's rows (4096 / 12288 of them: 64 x 128 results 24 / 60, 32 x 128 17 / 42, 16 x 128 13 / 30; 128 x
+# 256 72 / 200; 509 x 4096 x 4096 on 64 x 128 26, on 64 x 256 tiles 48)
+_GRAD = ([(xr, 128, (0, xr, 0), c, e) for xr, c, e in ((16, 0.133, 4.8), (32, 0.2, 4.2), (64, 0.28, 6.5))]
+         + [(32 * mj, 256, (1, mj, 2), c, e) for mj, c, e in ((4, 1.0, 6.0), (8, 1.42, 8.0))])
+
+
+@functools.lru_cache(4096)
+def _grad_form(M: int, N: int, K: int) -> tuple:
+    """(0, rows, 0) of the few-row kernel or (1, mj, wn) of the tiles for dy [M, N] against a weight [N, K]."""
+    return _best(M, K, N, _GRAD)
+
+
+@functools.lru_cache(4096)
+def _matmul_form(M: int, N: int) -> tuple:
+    return _best(M, N, 64, _MATMUL)
 
 
 # ---- products ---------------------------------------------------------------------------------------
 def _check(name: str, K: int, device, w, bias: Optional[torch.Tensor], dtype: torch.dtype) -> None:
-    if not isinstance(w, MXFP4):
+    if type(w) is not MXFP4:
         raise ValueError(f"{name}: the weight is no MXFP4 matrix (mxfp4_quantize makes one)")
     if w.shape[1] != K:
         raise ValueError(f"{name}: rows of {K} values against a weight of {w.shape[1]}")
-    if w.device != device:
+    if w.data.device != device:
         raise ValueError(f"{name}: rows on {device}, weight on {w.device}")
-    if bias is not None and (bias.dim() != 1 or bias.shape[0] != w.shape[0] or bias.dtype != dtype or bias.device != device):
-        raise ValueError(f"{name}: the bias is not [{w.shape[0]}] values of {dtype} on {device}")
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != w.shape[0] or bias.dtype != dtype or bias.device != device:
+            raise ValueError(f"{name}: the bias is not [{w.shape[0]}] values of {dtype} on {device}")
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name}: the bias has no gradient here (freeze it, or add it to the result)")
 
 
-def _linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor]) -> torch.Tensor:
+def _linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``mxfp4_linear`` of checked rows [M, K], without autograd."""
     (M, K), N = x.shape, w.shape[0]
     if not use_seqmix(x):
         y = x.float() @ _decode(w.codes, w.scales).to(x.dtype).float().t()
         return (y if bias is None else y + bias.float()).to(x.dtype)
-    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
     if M and N:
-        with _on(x.device):
-            x = _rows(x)
-            call("sm_mx_linear", DT[x.dtype], x, _ld(x), w._codes, w._scales, None if bias is None else bias.contiguous(), y, M, N, K, *_linear_tile(M, N))
+        x, p, ld = _rows(x)
+        if bias is not None:
+            bias = bias.contiguous()
+        tiles, m, n = _linear_form(M, N, K)
+        _launch("sm_mx_linear" if tiles else "sm_mx_rows", y.device, DT[x.dtype], p, ld, *_addresses(w), 0 if bias is None else bias.data_ptr(),
+                y.data_ptr(), M, N, K, m, n)
     return y
 
 
@@ -247,62 +301,63 @@ def _input_grad(dy: torch.Tensor, w: MXFP4) -> torch.Tensor:
         return (dy.float() @ _decode(w.codes, w.scales).to(dy.dtype).float()).to(dy.dtype)
     if not (M and N):
         return torch.zeros(M, K, dtype=dy.dtype, device=dy.device)
-    dx = torch.empty(M, K, dtype=dy.dtype, device=dy.device)
-    with _on(dy.device):
-        dy = F.pad(dy, (0, -N % 8)) if N % 8 else _rows(dy)          # (rows at 16-byte addresses, zeros behind them)
-        call("sm_mx_grad", DT[dy.dtype], dy, _ld(dy), w._codes, w._scales, dx, M, N, K, *_grad_tile(M, K))
+    dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
+    if N % 8:                                      # (rows at 16-byte addresses, zeros behind them)
+        dy = F.pad(dy, (0, -N % 8))
+    dy, p, ld = _rows(dy)
+    tiles, m, wn = _grad_form(M, N, K)
+    args = (DT[dy.dtype], p, ld, *_addresses(w), dx.data_ptr(), M, N, K, m)
+    if tiles:
+        _launch("sm_mx_grad", dx.device, *args, wn)
+    else:
+        _launch("sm_mx_rows_grad", dx.device, *args)
     return dx
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias):
-        ctx.save_for_backward(w._codes, w._scales)
-        ctx.K = w.shape[1]
+        ctx.save_for_backward(w.data)
+        ctx.shape = w.shape
         return _linear(x, w, bias)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        codes, scales = ctx.saved_tensors
-        return _input_grad(dy, _of(codes, scales, ctx.K)), None, None
+        return _input_grad(dy, _of(*ctx.saved_tensors, ctx.shape)), None, None
 
 
 def mxfp4_linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [..., K] @ W^T (+ ``bias`` [N]) for a weight [N, K] in MXFP4: W's values in x's type (``mxfp4_dequantize``), fp32
     sums, one rounding to x's type (bf16 or fp16; on the CPU fp32 too).  Differentiable in x, not in the weight or the bias."""
-    if x.dim() < 1 or x.dtype not in (DT if not x.is_cuda else HALF):
+    if x.dim() < 1 or x.dtype not in (HALF if x.is_cuda else DT):
         raise ValueError("mxfp4_linear: rows [..., K] of bf16 or fp16")
     K = x.shape[-1]
     _check("mxfp4_linear", K, x.device, w, bias, x.dtype)
-    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
-        raise ValueError("mxfp4_linear: the bias has no gradient here (freeze it, or add it to the result)")
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    if torch.is_grad_enabled() and x.requires_grad:
-        y = _Linear.apply(x2, w, bias)
-    else:
-        y = _linear(x2, w, bias)
+    if x2.shape[0] > MAX_ROWS:
+        raise ValueError(f"mxfp4_linear: {x2.shape[0]} rows (at most {MAX_ROWS})")
+    y = _Linear.apply(x2, w, bias) if x.requires_grad and torch.is_grad_enabled() else _linear(x2, w, bias)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
 
 
 def mxfp4_matmul(a: MXFP4, b: MXFP4, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a [M, K] @ b [N, K]^T (+ ``bias`` [N] of ``out_dtype``) of two MXFP4 matrices: fp32 sums of their exact products, one
     rounding to ``out_dtype`` (bf16, fp16 or fp32).  No gradient: activations that need one stay in 16 bits (``mxfp4_linear``)."""
-    if not isinstance(a, MXFP4):
+    if type(a) is not MXFP4:
         raise ValueError("mxfp4_matmul: the rows are no MXFP4 matrix (mxfp4_quantize makes one)")
     if out_dtype not in DT:
         raise ValueError("mxfp4_matmul: results in bf16, fp16 or fp32")
-    (M, K) = a.shape
-    _check("mxfp4_matmul", K, a.device, b, bias, out_dtype)
-    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
-        raise ValueError("mxfp4_matmul: the bias has no gradient here")
+    (M, K), dev = a.shape, a.data.device
+    _check("mxfp4_matmul", K, dev, b, bias, out_dtype)
     N = b.shape[0]
-    if not use_seqmix(a._codes):
+    if not use_seqmix(a.data):
         y = _decode(a.codes, a.scales) @ _decode(b.codes, b.scales).t()
         return (y if bias is None else y + bias.float()).to(out_dtype)
-    y = torch.empty(M, N, dtype=out_dtype, device=a.device)
+    y = torch.empty((M, N), dtype=out_dtype, device=dev)
     if M and N:
-        with _on(a.device):
-            call("sm_mx_matmul", DT[out_dtype], a._codes, a._scales, b._codes, b._scales,
-                 None if bias is None else bias.contiguous(), y, M, N, K, *_matmul_tile(M, N))
+        if bias is not None:
+            bias = bias.contiguous()
+        _launch("sm_mx_matmul", dev, DT[out_dtype], *_addresses(a), *_addresses(b), 0 if bias is None else bias.data_ptr(), y.data_ptr(),
+                M, N, K, *_matmul_form(M, N))
     return y

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import _ref_mxfp4 as ref
+import lumen.ops.mxfp4 as mx
 from lumen.ops.mxfp4 import MXFP4, mxfp4_dequantize, mxfp4_linear, mxfp4_matmul, mxfp4_quantize
 
 pytestmark = pytest.mark.gpu
@@ -165,6 +166,34 @@ def test_matmul_rows(M, dtype):
 @pytest.mark.parametrize("M,N,K", [(1, 2048, 4096), (48, 4100, 5632), (509, 1000, 2080), (1021, 2048, 544), (2050, 516, 1024), (1030, 4097, 288)])
 def test_matmul_sizes(M, N, K, dtype):
     check_matmul(M, N, K, dtype, bias=True)
+
+
+# every form of the kernels, at sizes that end inside its tiles and with fewer stages than its rings hold
+EDGES = [(1, 1, 32), (33, 100, 96), (70, 257, 192), (300, 515, 416), (129, 384, 2080)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("form", sorted({f[2] for f in mx._ROWS + mx._TILES}))
+def test_linear_forms(form, dtype, monkeypatch):
+    monkeypatch.setattr(mx, "_linear_form", lambda M, N, K: form)
+    for M, N, K in EDGES:
+        check_linear(M, N, K, dtype, bias=True)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("form", sorted({f[2] for f in mx._GRAD}))
+def test_grad_forms(form, dtype, monkeypatch):
+    monkeypatch.setattr(mx, "_grad_form", lambda M, N, K: form)
+    for M, K, N in EDGES:
+        check_grad(M, N, -(-K // 32) * 32, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, *HALF])
+@pytest.mark.parametrize("form", sorted({f[2] for f in mx._MATMUL}))
+def test_matmul_forms(form, dtype, monkeypatch):
+    monkeypatch.setattr(mx, "_matmul_form", lambda M, N: form)
+    for M, N, K in EDGES:
+        check_matmul(M, N, K, dtype, bias=True)
 
 
 @pytest.mark.parametrize("M", [3, 64, 300])
