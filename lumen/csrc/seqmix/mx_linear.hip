@@ -24,7 +24,7 @@ __global__ void __launch_bounds__(256, 1) linear_kernel(const TileArgs a) {
   }
 #pragma unroll
   for (int q = 0; q < S::PW; ++q)
-    offw[q] = (unsigned)column((wid + 4 * q) % S::NW * 32 + (lane & 31)) * 64u + 16 * (lane >> 5);
+    offw[q] = (unsigned)column((wid + 4 * q) % S::NW * 32 + (lane >> 1)) * 64u + 16 * ((lane ^ lane >> 4) & 1);
   offs = (unsigned)column(min(64 * wid + lane, S::BN - 1)) * 4u;
   const int nk = (a.K + 63) / 64;
   const mx::Walk walk{(const char*)a.x + (long long)m0 * a.ldx * 2, (const char*)a.codes, (const char*)a.scales, (long long)a.N * 64,

@@ -175,7 +175,7 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
         raw[n] = *reinterpret_cast<const unsigned*>(d + XB + wn * 4096 + h * 2048 + (4 * n + lg) * 64 + lr * 4);
       } else {
         const int r = wrow + 16 * n;
-        raw[n] = *reinterpret_cast<const unsigned*>(d + XB + (r >> 5) * 1024 + h * 512 + (r & 31) * 16 + lg * 4);
+        raw[n] = *reinterpret_cast<const unsigned*>(d + XB + r * 32 + (((h ^ lr >> 3) & 1) << 4) + lg * 4);
       }
     } else if (n < RW + RS) {
       const int u = n - RW;

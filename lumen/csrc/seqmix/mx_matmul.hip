@@ -29,6 +29,98 @@ __global__ void __launch_bounds__(256, 1) matmul_kernel(const TileArgs a) {
   mx::put_all<T, NI, MJ>(a, acc, m0 + 16 * MJ * (wid / WN), n0 + 16 * NI * (wid % WN));
 }
 
+// Few results: a workgroup takes XR rows and 16 RT columns, its four waves split k, each in a ring of its own (seqmix/mx_rows.hip); a
+// stage is a panel.
+template <int XR, int RT, int D>
+struct Ring {
+  static constexpr int NW = 4, MT = XR / 16, XB = MT * 1024, WB = RT * 1024, SX = (MT + 3) / 4, SW = (RT + 3) / 4;
+  static constexpr int SB = XB + WB + (SX + SW) * 256, G = MT + RT + SX + SW, PART = RT * MT * 1024;
+  static constexpr int LDS = NW * D * SB > NW * PART ? NW * D * SB : NW * PART;
+  static_assert(XR % 16 == 0 && LDS <= mx::kLds && D >= 2 && G * (D - 1) < 64, "ring");
+};
+
+template <typename T, int XR, int RT, int D>
+__global__ void __launch_bounds__(256, 1) rows_matmul_kernel(const TileArgs a) {
+  using S = Ring<XR, RT, D>;
+  constexpr int NW = S::NW, MT = S::MT, SX = S::SX, SW = S::SW, XB = S::XB, WB = S::WB, G = S::G;
+  __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = tile::unit_of(blockIdx.x, gridDim.x);
+  const int tm = tile % a.tiles_m, tn = tile / a.tiles_m;                // the row groups of a column tile share an XCD
+  const int m0 = tm * XR, n0 = tn * 16 * RT;
+  char* ring = lds + wid * D * S::SB;
+  const unsigned ring0 = __builtin_amdgcn_readfirstlane(mx::lds_addr(ring));
+  const int steps = (a.K + 127) / 128, t0 = steps * wid / NW, nk = steps * (wid + 1) / NW - t0;
+  const long long xp = (long long)a.M * 64, xsp = (long long)a.M * 4, wp = (long long)a.N * 64, sp = (long long)a.N * 4;
+  auto row = [&](int r) { return (unsigned)min(m0 + r, a.M - 1); };
+  auto column = [&](int r) { return (unsigned)min(n0 + r, a.N - 1); };
+  unsigned offx[MT], offw[RT], offxs[SX], offs[SW];
+#pragma unroll
+  for (int q = 0; q < MT; ++q) offx[q] = row(16 * q + (lane >> 2)) * 64u + 16 * (lane & 3);
+#pragma unroll
+  for (int q = 0; q < RT; ++q) offw[q] = column(16 * q + (lane >> 2)) * 64u + 16 * (lane & 3);
+#pragma unroll
+  for (int q = 0; q < SX; ++q) offxs[q] = row(64 * q + lane) * 4u;
+#pragma unroll
+  for (int q = 0; q < SW; ++q) offs[q] = column(64 * q + lane) * 4u;
+  auto issue = [&](int i) __attribute__((always_inline)) {
+    const int t = t0 + i;
+    const unsigned d = ring0 + i % D * S::SB;
+#pragma unroll
+    for (int q = 0; q < RT; ++q) tile::dma16((const char*)a.codes + t * wp, offw[q], __builtin_amdgcn_readfirstlane(d + XB + q * 1024));
+#pragma unroll
+    for (int q = 0; q < SW; ++q) mx::dma4((const char*)a.scales + t * sp, offs[q], __builtin_amdgcn_readfirstlane(d + XB + WB + (SX + q) * 256));
+#pragma unroll
+    for (int q = 0; q < SX; ++q) mx::dma4((const char*)a.xs + t * xsp, offxs[q], __builtin_amdgcn_readfirstlane(d + XB + WB + q * 256));
+#pragma unroll
+    for (int q = 0; q < MT; ++q) tile::dma16((const char*)a.x + t * xp, offx[q], __builtin_amdgcn_readfirstlane(d + q * 1024));
+  };
+  f32x4 acc[RT][MT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < D - 1; ++i)
+    if (i < nk) issue(i);
+  for (int i = 0; i < nk; ++i) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the fragments of stage i - 1 have been read: its slot may be filled again)
+    if (i + D - 1 < nk) issue(i + D - 1);
+    tile::wait_stages<D - 1, G>(nk - 1 - i);             // stage i has arrived
+    asm volatile("" ::: "memory");
+    const char* img = ring + i % D * S::SB;
+    uint4 x[MT];
+    unsigned sx[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      x[j] = *reinterpret_cast<const uint4*>(img + (16 * j + lr) * 64 + lg * 16);
+      sx[j] = *reinterpret_cast<const unsigned*>(img + XB + WB + (16 * j + lr) * 4) >> (8 * lg);
+    }
+#pragma unroll
+    for (int u = 0; u < RT; ++u) {
+      const uint4 w = *reinterpret_cast<const uint4*>(img + XB + (16 * u + lr) * 64 + lg * 16);
+      const unsigned sw = *reinterpret_cast<const unsigned*>(img + XB + WB + SX * 256 + (16 * u + lr) * 4) >> (8 * lg);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) mx::mfma4<false>(acc[u][j], w, x[j], sw, sx[j]);
+    }
+  }
+  // the waves' sums, over the rings
+  tile::done_reading();
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(lds + wid * S::PART + (i * MT + j) * 1024 + lane * 16) = acc[i][j];
+  __syncthreads();
+  for (int q = wid; q < RT * MT; q += NW) {
+    f32x4 v = *reinterpret_cast<const f32x4*>(lds + q * 1024 + lane * 16);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const f32x4*>(lds + w * S::PART + q * 1024 + lane * 16);
+    const int i = q / MT, m = m0 + 16 * (q - i * MT) + lr;
+    if (m < a.M) mx::put<T>(a, m, n0 + 16 * i + 4 * lg, false, v, v);
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -49,7 +141,33 @@ hipError_t sm_mx_matmul(int dt, const void* xc, const void* xs, const void* code
     else if (dt == kF16) matmul_kernel<fp16, NI, MJ, 2><<<grid, 256, 0, st>>>(a);      \
     else matmul_kernel<float, NI, MJ, 2><<<grid, 256, 0, st>>>(a);                     \
     break;
-    GO(1, 1) GO(1, 2) GO(1, 4) GO(1, 8) GO(2, 1) GO(2, 2) GO(2, 4) GO(2, 8) GO(4, 2) GO(4, 4) GO(4, 8) GO(8, 4) GO(8, 8)
+    GO(8, 4) GO(8, 8)
+#undef GO
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+// the same of few results: xr rows x 16 rt columns a workgroup
+hipError_t sm_mx_rows_matmul(int dt, const void* xc, const void* xs, const void* codes, const void* scales, const void* bias, void* y,
+                             int M, int N, int K, int xr, int rt, hipStream_t st) {
+  if (!mx::sizes_ok(M, N, K) || ((uintptr_t)xc | (uintptr_t)xs | (uintptr_t)codes | (uintptr_t)scales) % 16 ||
+      (dt != kF16 && dt != kBF16 && dt != kF32))
+    return hipErrorInvalidValue;
+  TileArgs a{xc, 0, xs, codes, scales, bias, y, M, N, K, 0, 0, 0, 0, mx::store_width(y, N, dt == kF32 ? 4 : 2)};
+  int grid;
+  if (!mx::plan(a, N, xr, 16 * rt, grid)) return hipErrorInvalidValue;
+  switch (10 * xr + rt) {
+#define GO(XR, RT, D)                                                                  \
+  case 10 * XR + RT:                                                                   \
+    if (dt == kBF16) rows_matmul_kernel<bf16, XR, RT, D><<<grid, 256, 0, st>>>(a);     \
+    else if (dt == kF16) rows_matmul_kernel<fp16, XR, RT, D><<<grid, 256, 0, st>>>(a); \
+    else rows_matmul_kernel<float, XR, RT, D><<<grid, 256, 0, st>>>(a);                \
+    break;
+    GO(16, 1, 8) GO(16, 2, 8) GO(16, 4, 6) GO(16, 6, 5) GO(16, 8, 4)
+    GO(32, 1, 8) GO(32, 2, 8) GO(32, 4, 6) GO(32, 6, 4) GO(32, 8, 3)
+    GO(64, 1, 6) GO(64, 2, 5) GO(64, 3, 5) GO(64, 4, 4) GO(64, 6, 3) GO(64, 8, 3)
+    GO(128, 4, 3)
 #undef GO
     default: return hipErrorInvalidValue;
   }

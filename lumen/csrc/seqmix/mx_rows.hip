@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_kernel(const TileArgs a) {
 #pragma unroll
   for (int q = 0; q < WP; ++q)
     offw[q] = KS == 128 ? (unsigned)min(n0 + 16 * q + (lane >> 2), a.N - 1) * 64u + 16 * (lane & 3)
-                        : (unsigned)min(n0 + 32 * q + (lane & 31), a.N - 1) * 64u + 16 * (lane >> 5);
+                        : (unsigned)min(n0 + 32 * q + (lane >> 1), a.N - 1) * 64u + 16 * ((lane ^ lane >> 4) & 1);
 #pragma unroll
   for (int q = 0; q < SP; ++q) offs[q] = (unsigned)min(n0 + 64 * q + lane, a.N - 1) * 4u;
   const int tail = a.K - KS * (steps - 1);               // values of x in the last stage
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_kernel(const TileArgs a) {
       } else {
 #pragma unroll
         for (int h = 0; h < NH; ++h)
-          raw[u][h] = *reinterpret_cast<const unsigned*>(img + XB + (u >> 1) * 1024 + h * 512 + (u & 1) * 256 + lr * 16 + lg * 4);
+          raw[u][h] = *reinterpret_cast<const unsigned*>(img + XB + u * 512 + lr * 32 + (((h ^ lr >> 3) & 1) << 4) + lg * 4);
       }
     }
     // KS 128: lane (lr, lg) multiplies k 32 lg + 8 h .. + 7 in step h; 64: k 32 h + 8 lg ..

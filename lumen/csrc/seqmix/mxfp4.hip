@@ -62,10 +62,8 @@ template <typename T> __device__ __forceinline__ unsigned codes8(const uint4 (&v
   return c;
 }
 
-// A workgroup: 16 rows by kPan panels, 16 lanes a row of a panel, four a block; a wave writes whole lines of four rows.
-constexpr int kPan = 4;
-
-template <typename T>
+// Bound by memory.  A workgroup: 16 rows by kPan panels, 16 lanes a row of a panel, four a block; a wave writes whole lines of four rows.
+template <typename T, int kPan>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, long long ldx, unsigned* __restrict__ codes,
                                                        unsigned char* __restrict__ scales, int R, int K, int panels) {
   const int r = blockIdx.x * 16 + (threadIdx.x >> 4), u = threadIdx.x & 15, p0 = blockIdx.y * kPan;
@@ -106,7 +104,7 @@ template <typename T> __device__ __forceinline__ void values8(unsigned c, float 
   }
 }
 
-template <typename T>
+template <typename T, int kPan>
 __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned* __restrict__ codes, const unsigned char* __restrict__ scales,
                                                          T* __restrict__ y, int R, int K, int panels) {
   const int r = blockIdx.x * 16 + (threadIdx.x >> 4), u = threadIdx.x & 15, p0 = blockIdx.y * kPan;
@@ -125,8 +123,12 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned* __restr
   }
 }
 
-// workgroups for R rows of K values
-inline dim3 grid_of(int R, int panels) { return dim3((R + 15) / 16, (panels + kPan - 1) / kPan); }
+// workgroups for R rows, `pan` panels each
+inline dim3 grid_of(int R, int panels, int pan) { return dim3((R + 15) / 16, (panels + pan - 1) / pan); }
+// Panels a workgroup takes: one of few values, whose loads then start at once everywhere, two of many, where half the workgroups come
+// and go (us, 1 / 2 / 4 panels: quantised 8 x 4096 2.0 / 2.0 / 2.2, 509 x 5632 3.4 / 3.6 / 4.0, 1021 x 5632 5.6 / 5.4 / 5.8, 22016 x 4096 50.0 /
+// 45.5 / 47.2 = 5.0 TB/s; back to 16 bits 2.0, 3.2 / 3.4 / 3.5, 5.2 / 4.9 / 5.1, 51.0 / 48.4 / 49.6).
+inline bool few(int R, int K) { return (long long)R * K <= (4 << 20); }
 
 }  // namespace
 
@@ -140,9 +142,12 @@ hipError_t sm_mx_quantize(int dt, const void* x, long long ldx, void* codes, voi
     return hipErrorInvalidValue;
   unsigned* c = (unsigned*)codes;
   unsigned char* s = (unsigned char*)scales;
-  if (dt == kF32) quantize_kernel<float><<<grid_of(R, P), 256, 0, st>>>((const float*)x, ldx, c, s, R, K, P);
-  else if (dt == kBF16) quantize_kernel<bf16><<<grid_of(R, P), 256, 0, st>>>((const bf16*)x, ldx, c, s, R, K, P);
-  else quantize_kernel<fp16><<<grid_of(R, P), 256, 0, st>>>((const fp16*)x, ldx, c, s, R, K, P);
+#define GO(PAN)                                                                                                                     \
+  if (dt == kF32) quantize_kernel<float, PAN><<<grid_of(R, P, PAN), 256, 0, st>>>((const float*)x, ldx, c, s, R, K, P);             \
+  else if (dt == kBF16) quantize_kernel<bf16, PAN><<<grid_of(R, P, PAN), 256, 0, st>>>((const bf16*)x, ldx, c, s, R, K, P);         \
+  else quantize_kernel<fp16, PAN><<<grid_of(R, P, PAN), 256, 0, st>>>((const fp16*)x, ldx, c, s, R, K, P);
+  if (few(R, K)) { GO(1) } else { GO(2) }
+#undef GO
   return hipGetLastError();
 }
 
@@ -154,9 +159,12 @@ hipError_t sm_mx_dequantize(int dt, const void* codes, const void* scales, void*
     return hipErrorInvalidValue;
   const unsigned* c = (const unsigned*)codes;
   const unsigned char* s = (const unsigned char*)scales;
-  if (dt == kF32) dequantize_kernel<float><<<grid_of(R, P), 256, 0, st>>>(c, s, (float*)y, R, K, P);
-  else if (dt == kBF16) dequantize_kernel<bf16><<<grid_of(R, P), 256, 0, st>>>(c, s, (bf16*)y, R, K, P);
-  else dequantize_kernel<fp16><<<grid_of(R, P), 256, 0, st>>>(c, s, (fp16*)y, R, K, P);
+#define GO(PAN)                                                                                                                     \
+  if (dt == kF32) dequantize_kernel<float, PAN><<<grid_of(R, P, PAN), 256, 0, st>>>(c, s, (float*)y, R, K, P);                      \
+  else if (dt == kBF16) dequantize_kernel<bf16, PAN><<<grid_of(R, P, PAN), 256, 0, st>>>(c, s, (bf16*)y, R, K, P);                  \
+  else dequantize_kernel<fp16, PAN><<<grid_of(R, P, PAN), 256, 0, st>>>(c, s, (fp16*)y, R, K, P);
+  if (few(R, K)) { GO(1) } else { GO(2) }
+#undef GO
   return hipGetLastError();
 }
 

@@ -240,11 +240,23 @@ def _best(M: int, N: int, K: int, forms) -> tuple:
 @functools.lru_cache(4096)
 def _linear_form(M: int, N: int, K: int) -> tuple:
     """(0, rows, 16 columns) of the few-row kernel or (1, mj, ni) of the tiles for x [M, K] against a weight [N, K]."""
-    return _best(M, N, K, _ROWS + _TILES if M > 64 else [f for f in _ROWS if f[0] >= min(M, 64)])
+    return _best(M, N, K, _ROWS + _TILES if M > 64 else [f for f in _ROWS if f[0] >= min(M, 16)])
 
 
-_MATMUL = [(32 * mj, 32 * ni, (mj, ni), max(mj * ni * 8, (mj + ni) * 23) + 100, 0)
-           for mj, ni in ((8, 8), (8, 4), (4, 8), (4, 4), (4, 2), (2, 8), (2, 4), (2, 2), (2, 1), (1, 8), (1, 4), (1, 2), (1, 1))]
+# both operands in 4 bits (64 x 16 results 6.2 / 11.5, 64 x 128 12 / 22, 128 x 64 11.7 / 22, 16 x 16 4.8 / 8; 256 x 128 33 / 72, 256 x 256 49 / 104)
+_MATMUL = ([(xr, 16 * rt, (0, xr, rt), (a + b * rt) / 2, f + g * rt)
+            for xr, a, b, f, g, rts in ((16, 0.05, 0.0125, 2.9, 0.1, (1, 2, 4, 6, 8)), (32, 0.05, 0.015, 3.3, 0.1, (1, 2, 4, 6, 8)),
+                                        (64, 0.087, 0.013, 2.8, 0.4, (1, 2, 3, 4, 6, 8)), (128, 0.0, 0.048, 0.0, 1.4, (4,)))
+            for rt in rts]
+           + [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.36, 10.0), (8, 0.515, 15.7))])
+
+
+@functools.lru_cache(4096)
+def _matmul_form(M: int, N: int, K: int) -> tuple:
+    """(0, rows, 16 columns) of the few-row kernel or (1, mj, ni) of the tiles."""
+    return _best(M, N, K, _MATMUL)
+
+
 # the gradient likewise, a stage 64 of the weight's rows (4096 / 12288 of them: 64 x 128 results 24 / 60, 32 x 128 17 / 42, 16 x 128 13 / 30; 128 x
 # 256 72 / 200; 509 x 4096 x 4096 on 64 x 128 26, on 64 x 256 tiles 48)
 _GRAD = ([(xr, 128, (0, xr, 0), c, e) for xr, c, e in ((16, 0.133, 4.8), (32, 0.2, 4.2), (64, 0.28, 6.5))]
@@ -255,11 +267,6 @@ _GRAD = ([(xr, 128, (0, xr, 0), c, e) for xr, c, e in ((16, 0.133, 4.8), (32, 0.
 def _grad_form(M: int, N: int, K: int) -> tuple:
     """(0, rows, 0) of the few-row kernel or (1, mj, wn) of the tiles for dy [M, N] against a weight [N, K]."""
     return _best(M, K, N, _GRAD)
-
-
-@functools.lru_cache(4096)
-def _matmul_form(M: int, N: int) -> tuple:
-    return _best(M, N, 64, _MATMUL)
 
 
 # ---- products ---------------------------------------------------------------------------------------
@@ -358,6 +365,7 @@ def mxfp4_matmul(a: MXFP4, b: MXFP4, bias: Optional[torch.Tensor] = None, out_dt
     if M and N:
         if bias is not None:
             bias = bias.contiguous()
-        _launch("sm_mx_matmul", dev, DT[out_dtype], *_addresses(a), *_addresses(b), 0 if bias is None else bias.data_ptr(), y.data_ptr(),
-                M, N, K, *_matmul_form(M, N))
+        tiles, m, n = _matmul_form(M, N, K)
+        _launch("sm_mx_matmul" if tiles else "sm_mx_rows_matmul", dev, DT[out_dtype], *_addresses(a), *_addresses(b),
+                0 if bias is None else bias.data_ptr(), y.data_ptr(), M, N, K, m, n)
     return y

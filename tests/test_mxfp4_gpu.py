@@ -191,7 +191,7 @@ def test_grad_forms(form, dtype, monkeypatch):
 @pytest.mark.parametrize("dtype", [torch.float32, *HALF])
 @pytest.mark.parametrize("form", sorted({f[2] for f in mx._MATMUL}))
 def test_matmul_forms(form, dtype, monkeypatch):
-    monkeypatch.setattr(mx, "_matmul_form", lambda M, N: form)
+    monkeypatch.setattr(mx, "_matmul_form", lambda M, N, K: form)
     for M, N, K in EDGES:
         check_matmul(M, N, K, dtype, bias=True)
 
