@@ -65,7 +65,7 @@ __device__ __forceinline__ void put_all(const TileArgs& a, f32x4 (&acc)[NI][MJ],
 }
 
 inline bool sizes_ok(int M, int N, int K) {
-  return M >= 1 && N >= 1 && M <= (1 << 24) && N <= (1 << 24) && K >= 32 && K % 32 == 0 && K <= (1 << 23);
+  return M >= 1 && N >= 1 && M <= (1 << 24) && N <= (1 << 24) && K >= 8 && K % 8 == 0 && K <= (1 << 23);
 }
 
 // grid of BM x BN tiles over M x C results; false: too many

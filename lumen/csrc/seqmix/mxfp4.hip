@@ -1,6 +1,6 @@
 // Microscaled 4-bit floating point (MXFP4): rows -> codes and scales, and back.
 //
-// A block is 32 values of a row.  Its scale is 2^e, e = floor(log2(max |x|)) - 2, kept as the byte e + 127; a value is the nearest
+// A block is 32 values of a row (the last one of a row the values that are left).  Its scale is 2^e, e = floor(log2(max |x|)) - 2, kept as the byte e + 127; a value is the nearest
 // of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} to x / 2^e, ties to the even code, 6 beyond.  Two values share a byte, the first in its low
 // half.  Blocks that hold an infinity or a NaN get the scale byte 255, which stands for NaN; blocks of zeros the byte 0.
 //  * floor(log2) is the exponent field of the largest magnitude (bit patterns of one sign compare like the numbers, NaN above all):
@@ -134,10 +134,10 @@ inline bool few(int R, int K) { return (long long)R * K <= (4 << 20); }
 
 extern "C" {
 
-// codes [panels, R, 64], scales [panels, R, 4] of x [R, K] at ldx; K % 32 == 0, panels of 128 values, rows of x at 16-byte addresses
+// codes [panels, R, 64], scales [panels, R, 4] of x [R, K] at ldx; K % 8 == 0, panels of 128 values, rows of x at 16-byte addresses
 hipError_t sm_mx_quantize(int dt, const void* x, long long ldx, void* codes, void* scales, int R, int K, hipStream_t st) {
   const int P = (K + 127) / 128;
-  if (R < 1 || R > (1 << 24) || K < 32 || K % 32 || K > (1 << 23) || ldx < K || ldx % (dt == kF32 ? 4 : 8) || (uintptr_t)x % 16 ||
+  if (R < 1 || R > (1 << 24) || K < 8 || K % 8 || K > (1 << 23) || ldx < K || ldx % (dt == kF32 ? 4 : 8) || (uintptr_t)x % 16 ||
       (uintptr_t)codes % 16 || (uintptr_t)scales % 4 || (dt != kF16 && dt != kBF16 && dt != kF32))
     return hipErrorInvalidValue;
   unsigned* c = (unsigned*)codes;
@@ -154,7 +154,7 @@ hipError_t sm_mx_quantize(int dt, const void* x, long long ldx, void* codes, voi
 // y [R, K] of such codes and scales
 hipError_t sm_mx_dequantize(int dt, const void* codes, const void* scales, void* y, int R, int K, hipStream_t st) {
   const int P = (K + 127) / 128;
-  if (R < 1 || R > (1 << 24) || K < 32 || K % 32 || K > (1 << 23) || (uintptr_t)y % 16 || (uintptr_t)codes % 16 || (uintptr_t)scales % 4 ||
+  if (R < 1 || R > (1 << 24) || K < 8 || K % 8 || K > (1 << 23) || (uintptr_t)y % 16 || (uintptr_t)codes % 16 || (uintptr_t)scales % 4 ||
       (dt != kF16 && dt != kBF16 && dt != kF32))
     return hipErrorInvalidValue;
   const unsigned* c = (const unsigned*)codes;

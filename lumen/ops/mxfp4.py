@@ -1,6 +1,6 @@
 """Microscaled 4-bit floating point (MXFP4): quantisation, and products with quantised operands.
 
-A row is cut into blocks of 32 values; a block holds one power of two, 2^e with e = floor(log2(largest magnitude)) - 2 (its
+A row is cut into blocks of 32 values (the last one holds what is left); a block holds one power of two, 2^e with e = floor(log2(largest magnitude)) - 2 (its
 byte is e + 127), and 32 four-bit numbers: +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}, the nearest to value / 2^e (ties to the even
 code, 6 beyond it).  Two share a byte, the first in its low half.  A block with an infinity or a NaN becomes NaN (byte 255).
 
@@ -31,7 +31,7 @@ HALF = (torch.bfloat16, torch.float16)
 
 
 class MXFP4:
-    """A matrix [rows, K] in MXFP4: ``codes`` uint8 [rows, K / 2], ``scales`` uint8 [rows, K / 32].
+    """A matrix [rows, K] in MXFP4, K a multiple of 8: ``codes`` uint8 [rows, K / 2], ``scales`` uint8 [rows, K / 32 rounded up].
 
     Built from such tensors (of another program's checkpoint, say) or by ``mxfp4_quantize``.  It holds them as the kernels read
     them, in panels of 128 values of all rows: [panel, row, 64] bytes of codes, then [panel, row, 4] of scales, zeros behind a
@@ -41,12 +41,12 @@ class MXFP4:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
-            raise ValueError("MXFP4: codes [rows, K / 2] and scales [rows, K / 32], both uint8")
+            raise ValueError("MXFP4: codes [rows, K / 2] and scales [rows, K / 32 rounded up], both uint8")
         R, K = codes.shape[0], 2 * codes.shape[1]
-        if scales.shape[0] != R or scales.shape[1] * BLOCK != K:
+        if scales.shape[0] != R or scales.shape[1] != -(-K // BLOCK):
             raise ValueError(f"MXFP4: scales {list(scales.shape)} do not fit codes {list(codes.shape)}")
-        if not 0 < K <= MAX_K or R > MAX_ROWS:
-            raise ValueError(f"MXFP4: {R} rows of {K} values (at most {MAX_ROWS}, and 32 to {MAX_K})")
+        if K % 8 or not 0 < K <= MAX_K or R > MAX_ROWS:
+            raise ValueError(f"MXFP4: {R} rows of {K} values (at most {MAX_ROWS}; a multiple of 8, at most {MAX_K})")
         if codes.device != scales.device:
             raise ValueError(f"MXFP4: codes on {codes.device}, scales on {scales.device}")
         self.shape = (R, K)
@@ -72,7 +72,7 @@ class MXFP4:
 
     @property
     def scales(self) -> torch.Tensor:
-        return _rows_of(self._scales)[:, :self.shape[1] // BLOCK]
+        return _rows_of(self._scales)[:, :-(-self.shape[1] // BLOCK)]
 
     @property
     def device(self) -> torch.device:
@@ -83,7 +83,7 @@ class MXFP4:
         return self.data.numel()
 
     def to(self, device) -> "MXFP4":
-        return _of(self.data.to(device), self.shape)
+        return of_data(self.data.to(device), self.shape)
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         return mxfp4_dequantize(self, dtype)
@@ -111,7 +111,8 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
     return t.transpose(0, 1).reshape(R, P * unit)
 
 
-def _of(data: torch.Tensor, shape: tuple) -> MXFP4:
+def of_data(data: torch.Tensor, shape: tuple) -> MXFP4:
+    """The [rows, K] matrix whose ``data`` this is."""
     q = MXFP4.__new__(MXFP4)
     q.data, q.shape = data, shape
     return q
@@ -159,16 +160,16 @@ def _launch(name: str, device: torch.device, *args) -> None:
 
 # ---- the format -------------------------------------------------------------------------------------
 def mxfp4_quantize(x: torch.Tensor) -> MXFP4:
-    """The MXFP4 form of x [rows, K] (fp32, bf16 or fp16; K a multiple of 32)."""
+    """The MXFP4 form of x [rows, K] (fp32, bf16 or fp16; K a multiple of 8)."""
     if x.dim() != 2 or x.dtype not in DT:
         raise ValueError("mxfp4_quantize: a matrix [rows, K] of fp32, bf16 or fp16")
     R, K = x.shape
-    if K % BLOCK or not 0 < K <= MAX_K or R > MAX_ROWS:
-        raise ValueError(f"mxfp4_quantize: {R} rows of {K} values (at most {MAX_ROWS}; a multiple of {BLOCK}, at most {MAX_K})")
+    if K % 8 or not 0 < K <= MAX_K or R > MAX_ROWS:
+        raise ValueError(f"mxfp4_quantize: {R} rows of {K} values (at most {MAX_ROWS}; a multiple of 8, at most {MAX_K})")
     if not use_seqmix(x):
         return MXFP4(*_encode(x.detach()))
     dev, dt = x.device, DT[x.dtype]
-    q = _of(torch.empty(_nbytes(R, K), dtype=torch.uint8, device=dev), (R, K))
+    q = of_data(torch.empty(_nbytes(R, K), dtype=torch.uint8, device=dev), (R, K))
     if R:
         x, p, ld = _rows(x.detach() if x.requires_grad else x, 8 if dt else 4)
         _launch("sm_mx_quantize", dev, dt, p, ld, *_addresses(q), R, K)
@@ -201,7 +202,8 @@ def _power(s: torch.Tensor) -> torch.Tensor:
 
 def _encode(x: torch.Tensor):
     R, K = x.shape
-    b = x.float().reshape(R, K // BLOCK, BLOCK)
+    n = -(-K // BLOCK)
+    b = F.pad(x.float(), (0, n * BLOCK - K)).reshape(R, n, BLOCK)
     top = b.abs().amax(-1)
     bad = ~torch.isfinite(b).all(-1)
     e = (top.contiguous().view(torch.int32) >> 23) - 2             # (exponent field: 0 of zero and denormals)
@@ -211,15 +213,16 @@ def _encode(x: torch.Tensor):
     step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0))
     r = (torch.round(a / step) * step).clamp(max=6.0)
     code = torch.where(r < 2, r * 2, torch.where(r < 4, r + 2, r / 2 + 4)).to(torch.uint8) | (torch.signbit(m).to(torch.uint8) << 3)
-    code = torch.where(bad.unsqueeze(-1), torch.zeros_like(code), code).reshape(R, K // 2, 2)
+    code = torch.where(bad.unsqueeze(-1), torch.zeros_like(code), code).reshape(R, n * BLOCK)[:, :K].reshape(R, K // 2, 2)
     return code[..., 0] | code[..., 1] << 4, s.to(torch.uint8)
 
 
 def _decode(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     lut = torch.tensor(_VALUES, dtype=torch.float32, device=codes.device)
-    R, n = scales.shape
-    v = torch.stack((lut[(codes & 15).long()], lut[(codes >> 4).long()]), -1).reshape(R, n, BLOCK)
-    return (v * _power(scales).unsqueeze(-1)).reshape(R, n * BLOCK)
+    (R, n), K = scales.shape, 2 * codes.shape[1]
+    v = torch.stack((lut[(codes & 15).long()], lut[(codes >> 4).long()]), -1).reshape(R, K)
+    v = F.pad(v, (0, n * BLOCK - K)).reshape(R, n, BLOCK)
+    return (v * _power(scales).unsqueeze(-1)).reshape(R, n * BLOCK)[:, :K]
 
 
 # What a round of 256 workgroups takes, us (bf16, weights from HBM): (a + b rt) a stage of 64 k and (f + g rt) beside them on the
@@ -284,7 +287,7 @@ def _check(name: str, K: int, device, w, bias: Optional[torch.Tensor], dtype: to
             raise ValueError(f"{name}: the bias has no gradient here (freeze it, or add it to the result)")
 
 
-def _linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+def linear_rows(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``mxfp4_linear`` of checked rows [M, K], without autograd."""
     (M, K), N = x.shape, w.shape[0]
     if not use_seqmix(x):
@@ -301,7 +304,7 @@ def _linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) -> t
     return y
 
 
-def _input_grad(dy: torch.Tensor, w: MXFP4) -> torch.Tensor:
+def input_grad(dy: torch.Tensor, w: MXFP4) -> torch.Tensor:
     """dx [M, K] = dy [M, N] times the weight's values in dy's type."""
     (M, N), K = dy.shape, w.shape[1]
     if not use_seqmix(dy):
@@ -326,12 +329,27 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, w, bias):
         ctx.save_for_backward(w.data)
         ctx.shape = w.shape
-        return _linear(x, w, bias)
+        return linear_rows(x, w, bias)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return _input_grad(dy, _of(*ctx.saved_tensors, ctx.shape)), None, None
+        w = of_data(*ctx.saved_tensors, ctx.shape)
+        twice = dy.requires_grad and torch.is_grad_enabled()
+        return _InputGrad.apply(dy, w) if twice else input_grad(dy, w), None, None
+
+
+class _InputGrad(torch.autograd.Function):
+    """The gradient, where it is to be differentiated once more."""
+
+    @staticmethod
+    def forward(ctx, dy, w):
+        ctx.save_for_backward(w.data)
+        ctx.shape = w.shape
+        return input_grad(dy, w)
+
+    @staticmethod
+    def backward(ctx, g):
+        return mxfp4_linear(g, of_data(*ctx.saved_tensors, ctx.shape)), None
 
 
 def mxfp4_linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -344,7 +362,7 @@ def mxfp4_linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None)
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     if x2.shape[0] > MAX_ROWS:
         raise ValueError(f"mxfp4_linear: {x2.shape[0]} rows (at most {MAX_ROWS})")
-    y = _Linear.apply(x2, w, bias) if x.requires_grad and torch.is_grad_enabled() else _linear(x2, w, bias)
+    y = _Linear.apply(x2, w, bias) if x.requires_grad and torch.is_grad_enabled() else linear_rows(x2, w, bias)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
 
 

@@ -7,9 +7,12 @@ MAGS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
 def encode(x):
-    """(codes [R, K], scale bytes [R, K / 32]) of x [R, K] as integers: for every value the nearest magnitude, of two the even code."""
-    R, K = x.shape
-    b = x.double().cpu().reshape(R, K // 32, 32)
+    """(codes [R, K], scale bytes [R, K / 32 rounded up]) of x [R, K] as integers: for every value the nearest magnitude, of two the even code."""
+    R, K0 = x.shape
+    K = -(-K0 // 32) * 32
+    b = torch.zeros(R, K, dtype=torch.float64)            # (a last block of fewer values: as if zeros followed)
+    b[:, :K0] = x.double().cpu()
+    b = b.reshape(R, K // 32, 32)
     top = b.abs().amax(-1)
     bad = ~torch.isfinite(b).all(-1)
     byte = torch.zeros_like(top, dtype=torch.long)
@@ -30,7 +33,7 @@ def encode(x):
     pick = torch.where(even, (near & (idx % 2 == 0)).double().argmax(-1), first)
     code = pick + 8 * torch.signbit(m).long()
     code = torch.where(bad.unsqueeze(-1), torch.zeros_like(code), code)
-    return code.reshape(R, K), byte
+    return code.reshape(R, K)[:, :K0], byte
 
 
 def decode(code, byte):
@@ -39,7 +42,7 @@ def decode(code, byte):
     v = torch.where(code >= 8, -mag, mag)
     unit = torch.pow(2.0, (byte - 127).double())
     unit = torch.where(byte == 255, torch.full_like(unit, float("nan")), unit)
-    return v * unit.repeat_interleave(32, 1)
+    return v * unit.repeat_interleave(32, 1)[:, :v.shape[1]]
 
 
 def unpack(q):

@@ -8,12 +8,12 @@ from lumen.ops.mxfp4 import MXFP4, mxfp4_dequantize, mxfp4_linear, mxfp4_matmul,
 
 def spread(R, K, seed, dtype=torch.float32):
     g = torch.Generator().manual_seed(seed)
-    x = torch.randn(R, K, generator=g) * torch.exp(4 * torch.randn(R, K // 32, generator=g)).repeat_interleave(32, 1)
+    x = torch.randn(R, K, generator=g) * torch.exp(4 * torch.randn(R, K // 8, generator=g)).repeat_interleave(8, 1)
     return x.to(dtype)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("R,K", [(1, 32), (3, 96), (7, 256)])
+@pytest.mark.parametrize("R,K", [(1, 32), (3, 96), (7, 256), (2, 8), (3, 104)])
 def test_format(R, K, dtype):
     x = spread(R, K, R + K, dtype).clamp(-60000, 60000)
     x[0, :32] = 0
@@ -48,10 +48,10 @@ def test_extremes():
     assert y[1, 3] == 6 * 2.0 ** 125 and y[4, 3] == 2.0 ** -126 and y[5, 3] == 6
 
 
-@pytest.mark.parametrize("K", [32, 96, 128, 416])
+@pytest.mark.parametrize("K", [8, 32, 96, 120, 128, 416])
 def test_rows_are_padded_and_given_back(K):
     q = mxfp4_quantize(spread(5, K, K))
-    assert q.codes.shape == (5, K // 2) and q.scales.shape == (5, K // 32)
+    assert q.codes.shape == (5, K // 2) and q.scales.shape == (5, -(-K // 32))
     again = MXFP4(q.codes.clone(), q.scales.clone())
     assert again.shape == q.shape
     assert torch.equal(mxfp4_dequantize(again), mxfp4_dequantize(q))
@@ -109,8 +109,9 @@ def test_refusals():
     refused(MXFP4, u8(4, 32), u8(3, 2))
     refused(MXFP4, u8(4, 32).view(-1), u8(4, 2))
     refused(MXFP4, u8(4, 0), u8(4, 0))
-    refused(MXFP4, u8(4, 24), u8(4, 2))
-    refused(mxfp4_quantize, torch.randn(3, 48))
+    refused(MXFP4, u8(4, 24), u8(4, 3))
+    refused(MXFP4, u8(4, 18), u8(4, 2))
+    refused(mxfp4_quantize, torch.randn(3, 60))
     refused(mxfp4_quantize, torch.randn(64))
     refused(mxfp4_quantize, torch.randn(3, 0))
     refused(mxfp4_quantize, torch.randn(3, 64).double())
