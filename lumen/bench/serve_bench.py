@@ -38,6 +38,7 @@ def make_engine(a):
                        max_num_seqs=a.max_num_seqs, max_num_batched_tokens=a.max_batched_tokens,
                        prefill_boost=a.prefill_boost, use_graphs=not a.no_graphs, init="random",
                        async_scheduling=not a.sync_scheduling, kv_cache_dtype=a.kv_cache_dtype,
+                       quantization=getattr(a, "quantization", None),
                        tp_size=getattr(a, "tp", 1),
                        scheduling_policy=getattr(a, "scheduling_policy", "chunked"),
                        num_blocks=getattr(a, "num_blocks", None),
@@ -273,6 +274,7 @@ def main():
                     help="x token budget while at most max-num-seqs/4 sequences decode (1: off)")
     ap.add_argument("--no-graphs", action="store_true")
     ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"])
+    ap.add_argument("--quantization", default=None, choices=[None, "mxfp4"])
     ap.add_argument("--sync-scheduling", action="store_true",
                     help="engine mode: host waits for each step's tokens before the next step")
     ap.add_argument("--tp", type=int, default=1,

@@ -101,6 +101,9 @@ def build_parser(variant: str) -> argparse.ArgumentParser:
                     help="same as --gradient_checkpointing false")
     ap.add_argument("--no_fuse_accumulation", action="store_true",
                     help="run every accumulation micro-batch as its own forward / backward")
+    ap.add_argument("--base_quantization", default=None, choices=[None, "mxfp4"],
+                    help="hold the frozen base weights in 4-bit floating point (MXFP4: 4.25 bits a "
+                         "value) under the adapters; ZeRO stages 0 - 2")
     ap.add_argument("--metrics_csv", default="results/training_metrics.csv")
     return ap
 
@@ -162,7 +165,8 @@ def main(variant: str, argv=None) -> dict:
         synthetic_samples=args.synthetic_samples, init=args.init, experiment=experiment,
         synthetic_min_len=args.synthetic_min_len, pack_sequences=not args.no_packing,
         prefetch=args.prefetch, pack_tokens=args.pack_tokens,
-        fuse_accumulation=not args.no_fuse_accumulation)
+        fuse_accumulation=not args.no_fuse_accumulation,
+        base_quantization=args.base_quantization)
     t0 = time.time()
     trainer = Trainer(targs, ds, env)
     result = trainer.train()

@@ -69,6 +69,27 @@ def apply_lora(model: nn.Module, cfg: LoraConfig) -> nn.Module:
     return model
 
 
+def quantize_base(model: nn.Module, how: str = "mxfp4") -> int:
+    """Hold the frozen weights of every projection but the LM head in 4 bits (``ops/mxfp4.py``); adapters, norms, embeddings
+    and biases stay as they are.  Llama and OPT models, before the engine is built, ZeRO stages 0 - 2.  Returns the number of
+    bytes that this frees."""
+    if how != "mxfp4":
+        raise ValueError(f"quantize_base: only 'mxfp4', got {how!r}")
+    lins = [(n, m) for n, m in model.named_modules() if isinstance(m, Linear) and not n.endswith("lm_head")]
+    if not lins:
+        raise ValueError("quantize_base: the model has no projections to quantise (Llama and OPT models)")
+    for n, m in lins:
+        if m.qdata is None and (m.in_features % 8 or m.weight.requires_grad):
+            raise ValueError(f"quantize_base: {n} ({m.in_features} inputs) is trainable, or its rows no multiple of 8")
+    freed = 0
+    for _, m in lins:
+        if m.qdata is None:
+            freed += m.weight.numel() * m.weight.element_size()
+            m.quantize_base()
+            freed -= m.qdata.numel()
+    return freed
+
+
 def count_parameters(model: nn.Module):
     trainable = sum(p.numel() for p in model.parameters() if p.requires_grad)
     total = 0

@@ -16,6 +16,7 @@ import torch.nn as nn
 
 from ..ops import lora as lora_ops
 from ..ops.lora import lora_linear, linear
+from ..ops.mxfp4 import MXFP4, mxfp4_quantize, of_data
 from ..ops.transpose import transpose_2d
 from ..ops.norm import rms_norm
 
@@ -70,6 +71,7 @@ class Linear(nn.Module):
                                    requires_grad=False)
         self.bias = (nn.Parameter(torch.zeros(out_features, dtype=dtype, device=device),
                                   requires_grad=False) if bias else None)
+        self.register_buffer("qdata", None, persistent=False)  # the weight in MXFP4 (quantize_base)
         self.seg_sizes = list(seg_sizes) if seg_sizes else [out_features]
         self.seg_names = list(seg_names) if seg_names else ["proj"]
         self.lora: Optional[LoRAAdapter] = None
@@ -82,8 +84,37 @@ class Linear(nn.Module):
         self._wext_key = None
         self._tail_key = None
 
-    def weight_fn(self) -> torch.Tensor:
-        return self.weight
+    @property
+    def qweight(self) -> Optional[MXFP4]:
+        """The base weight in MXFP4, or None where it is held in ``weight``."""
+        return None if self.qdata is None else of_data(self.qdata, (self.out_features, self.in_features))
+
+    @torch.no_grad()
+    def quantize_base(self) -> None:
+        """Hold the frozen base weight in MXFP4 (4.25 bits a value) from here on; ``weight`` becomes
+        empty.  Adapters on it train and run as before, on the quantised values."""
+        W = self.weight
+        if self.qdata is not None:
+            return
+        if W.requires_grad:
+            raise ValueError("quantize_base: the weight is trainable (freeze it, or apply adapters first)")
+        if W.dim() != 2 or getattr(W, "_lumen_gathered", False):
+            raise ValueError("quantize_base: the weight is partitioned (ZeRO-3): quantise at stages 0 - 2")
+        self.qdata = mxfp4_quantize(W).data
+        self.weight = nn.Parameter(W.new_empty(0), requires_grad=False)
+        self.weight._zero_shape = W.shape  # (parameter counts go by it)
+        self.invalidate_weight_cache()
+
+    @torch.no_grad()
+    def dequantize_base(self) -> None:
+        """Back to a 16-bit (or fp32) ``weight``, of the quantised values."""
+        if self.qdata is not None:
+            self.weight = nn.Parameter(self.qweight.dequantize(self.weight.dtype), requires_grad=False)
+            self.qdata = None
+            self.invalidate_weight_cache()
+
+    def weight_fn(self):
+        return self.weight if self.qdata is None else self.qweight
 
     def weight_t_fn(self) -> Optional[torch.Tensor]:
         """Contiguous W^T [in, out] for the backward dX = dY @ W, or None.
@@ -94,7 +125,7 @@ class Linear(nn.Module):
         gathered weights change storage every step: they are transposed on the fly, and only
         where the GEMM saving beats the transpose's HBM traffic (``transpose_gathered``)."""
         W = self.weight
-        if not self.transpose_bwd or W.requires_grad:
+        if not self.transpose_bwd or W.requires_grad or self.qdata is not None:
             return None
         if getattr(W, "_lumen_gathered", False):
             wt = getattr(W, "_lumen_wt", None)  # transposed by the ZeRO-3 coordinator off-path
@@ -239,10 +270,12 @@ class Linear(nn.Module):
 
     @torch.no_grad()
     def merge_lora(self):
-        """W += scale * B A for every adapted segment (serving: merge-on-load)."""
+        """W += scale * B A for every adapted segment (serving: merge-on-load).  A quantised
+        base is brought back to its 16-bit values first: the sum is not rounded to 4 bits."""
         lo = self.lora
         if lo is None:
             return
+        self.dequantize_base()
         W = self.weight
         for (n_off, n_len, r_off, b_off) in lo.segs:
             A = lo.lora_A[r_off:r_off + lo.r].float()

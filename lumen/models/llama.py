@@ -126,11 +126,11 @@ class LlamaMLP(nn.Module):
 
     @property
     def recompute_eligible(self) -> bool:
-        """Selective recompute needs frozen gate|up / down weights without active adapters
+        """Selective recompute needs frozen 16-bit gate|up / down weights without active adapters
         (``recompute_mlp`` re-runs only the frozen gate|up GEMM in the backward)."""
         gu, dn = self.gate_up_proj, self.down_proj
         return not (gu.has_active_lora or dn.has_active_lora or gu.weight.requires_grad
-                    or dn.weight.requires_grad)
+                    or dn.weight.requires_grad or gu.qdata is not None or dn.qdata is not None)
 
     def forward(self, x2d):
         gu, dn = self.gate_up_proj, self.down_proj
@@ -196,8 +196,8 @@ class LlamaForCausalLM(nn.Module):
         saving both scale with N, so ``--gradient_checkpointing auto`` recomputes just the
         layers the HBM budget needs (``memory_plan.pick_checkpointing``).
 
-        A layer whose MLP cannot use the selective recompute (trainable gate|up / down weights,
-        or adapters on them) is checkpointed whole instead (``full`` for that layer), so asking
+        A layer whose MLP cannot use the selective recompute (trainable or 4-bit gate|up / down
+        weights, or adapters on them) is checkpointed whole instead (``full`` for that layer), so asking
         for checkpointing never silently keeps every activation."""
         n = self._ckpt_layers
         return self._ckpt if n is None or self._ckpt == "none" else f"{self._ckpt}:{n}"
@@ -213,7 +213,7 @@ class LlamaForCausalLM(nn.Module):
             if not getattr(self, "_warned_selective", False):
                 self._warned_selective = True
                 import sys
-                print("[lumen] selective checkpointing: MLP weights are trainable or adapted, "
+                print("[lumen] selective checkpointing: MLP weights are trainable, adapted or in 4 bits, "
                       "those layers fall back to full per-layer recompute", file=sys.stderr)
             return "full"
         return self._ckpt

@@ -120,6 +120,8 @@ def save_hf_weights(model: nn.Module, path: str, shard_bytes: int = 5 << 30) -> 
             json.dump(to_dict(cfg), f, indent=2)
         return
     params = dict(model.named_parameters())
+    params.update({f"{n}.weight": m.qweight.dequantize(m.weight.dtype) for n, m in model.named_modules()
+                   if getattr(m, "qdata", None) is not None})        # (4-bit bases are written as 16-bit values)
     out: Dict[str, torch.Tensor] = {}
     for ours, srcs in _hf_name_map(model).items():
         if ours not in params:

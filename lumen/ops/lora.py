@@ -23,6 +23,8 @@ import torch.nn.functional as F
 
 from ._native import DTYPE_CODE, native, use_native
 from .gemm import matmul_nt, mm_nt
+from .mxfp4 import MXFP4, mxfp4_linear
+from .mxfp4 import input_grad as _mx_input_grad, linear_rows as _mx_linear
 
 Seg = Tuple[int, int, int, int]
 
@@ -526,7 +528,7 @@ class _LoraLinear(torch.autograd.Function):
         W = weight_fn() if fold is None else None
 
         def gemm():
-            y_ = matmul_nt(x2d, W)
+            y_ = matmul_nt(x2d, W) if type(W) is not MXFP4 else _mx_linear(x2d, W)
             if bias is not None:
                 y_.add_(bias)
             return y_
@@ -599,7 +601,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2d, weight_fn, bias, w_param, wt_fn):
         W = weight_fn()
-        y = mm_nt(x2d, W)
+        y = mm_nt(x2d, W) if type(W) is not MXFP4 else _mx_linear(x2d, W)
         if bias is not None:
             y.add_(bias)
         ctx.weight_fn = weight_fn
@@ -633,7 +635,8 @@ def _input_grad(ctx, dy):
     Wt = ctx.wt_fn() if ctx.wt_fn is not None else None
     if Wt is not None:
         return mm_nt(dy, Wt)
-    return torch.matmul(dy, ctx.weight_fn())
+    W = ctx.weight_fn()
+    return torch.matmul(dy, W) if type(W) is not MXFP4 else _mx_input_grad(dy, W)
 
 
 def linear(x: torch.Tensor, weight_fn, bias: Optional[torch.Tensor] = None,
@@ -643,16 +646,21 @@ def linear(x: torch.Tensor, weight_fn, bias: Optional[torch.Tensor] = None,
     if use_native(x2d):
         y = _Linear.apply(x2d.contiguous(), weight_fn, bias, w_param, wt_fn)
     else:
-        y = F.linear(x2d, _frozen(weight_fn()), bias)
+        y = _base(x2d, _frozen(weight_fn()), bias)
     # 2-D in -> return the Function output itself (not a view): a view would make a later
     # in-place op on it (RoPE on the fused QKV buffer) go through autograd's CopySlices
     return y if x.dim() == 2 else y.view(*shp[:-1], y.shape[-1])
 
 
-def _frozen(W: torch.Tensor) -> torch.Tensor:
+def _base(x2d, W, bias):
+    """The torch path of the base product, W in x's type or in MXFP4."""
+    return F.linear(x2d, W, bias) if type(W) is not MXFP4 else mxfp4_linear(x2d, W, bias)
+
+
+def _frozen(W):
     # autograd must not save the Parameter object itself: ZeRO-3 swaps param.data when it
     # releases a gathered unit; a detached alias keeps the gathered storage alive instead
-    return W if W.requires_grad else W.detach()
+    return W if type(W) is MXFP4 or W.requires_grad else W.detach()
 
 
 def lora_linear(x: torch.Tensor, weight_fn, bias: Optional[torch.Tensor], A: torch.Tensor,
@@ -693,7 +701,7 @@ def _rope_ref_cols(y: torch.Tensor, rope) -> torch.Tensor:
 
 
 def lora_linear_ref(x2d, W, bias, A, B, segs, r, scale, p, seed):
-    y = F.linear(x2d, W, bias)
+    y = _base(x2d, W, bias)
     xd = _apply_dropout_ref(x2d, p, seed)
     Z = xd.float() @ A.float().t()
     parts = []

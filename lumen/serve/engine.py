@@ -65,6 +65,9 @@ class EngineConfig:
     # KV-cache element type: "auto" = model dtype; "fp8" = e4m3 (vLLM --kv-cache-dtype fp8):
     # twice the cache capacity and half the K/V bytes per decode step, at fp8 K/V precision
     kv_cache_dtype: str = "auto"
+    # projections in 4-bit floating point ("mxfp4", made from the 16-bit weights at start; vLLM --quantization): 4.25 bits
+    # a weight instead of 16.  LM head, embeddings, norms and adapters keep the model dtype
+    quantization: Optional[str] = None
     # automatic prefix caching (vLLM --enable-prefix-caching): prompts share the cached K/V of
     # equal leading full blocks; finished sequences' blocks stay cached until evicted
     enable_prefix_caching: bool = False
@@ -142,6 +145,11 @@ class LLMEngine:
 
             load_tuned_gemms()  # tuned hipBLASLt algorithms for the prefill/decode GEMM shapes
         dt = _DT[cfg.dtype] if dev.type == "cuda" else torch.float32
+        if cfg.quantization not in (None, "mxfp4"):
+            raise ValueError(f"quantization must be None or 'mxfp4', got {cfg.quantization!r}")
+        if cfg.quantization and dev.type == "cuda" and dt == torch.float32:
+            raise ValueError("quantization: dtype bf16 or fp16 on the GPU")
+        own_model = model is None
         if model is None:
             model = build_model(cfg.model, dtype=dt, device=dev, init=cfg.init, seed=cfg.seed)
         if cfg.adapter:
@@ -165,7 +173,7 @@ class LLMEngine:
 
             self.weights = WEIGHTS[model.config.arch](model, self.rank, self.tp)
         else:
-            self.weights = ServeWeights(model, self.rank, self.tp)
+            self.weights = ServeWeights(model, self.rank, self.tp, cfg.quantization, own_model)
         limit = getattr(self.weights, "max_positions", None)
         if limit is not None and cfg.max_model_len > limit:
             # a learned position table ends there: no sequence may grow past its last row
@@ -254,6 +262,7 @@ class LLMEngine:
                                ("num_speculative_tokens", c.num_speculative_tokens > 0),
                                ("lora_modules", bool(c.lora_modules)),
                                ("adapter", bool(c.adapter)),
+                               ("quantization", c.quantization is not None),
                                ("kv_cache_dtype fp8", c.kv_cache_dtype == "fp8")) if on]
         if bad:
             raise ValueError(f"not supported for hybrid (recurrent-state) models: {', '.join(bad)}")

@@ -37,6 +37,7 @@ from ..ops.attention import (flash_attention_fresh, flash_attention_paged, paged
                              rope_write_kv)
 from ..ops.gemm import decoded_rows, linear_nt, row_norm_linear, row_norm_ok, swiglu_linear_nt
 from ..ops.moe import MID_MAX_M, THIN_ACT_MAX_M, mid_act, mid_act_ok, thin_act, thin_act_ok, tile_act, tile_act_ok
+from ..ops.mxfp4 import mxfp4_linear, mxfp4_quantize
 from ..ops.norm import rms_norm
 from ..ops.rope import rope_tables
 
@@ -96,10 +97,22 @@ class LayerW:
     down: torch.Tensor
 
 
+def _values(lin) -> torch.Tensor:
+    """A projection's weight, of a 4-bit base its values."""
+    return lin.weight if lin.qdata is None else lin.qweight.dequantize(lin.weight.dtype)
+
+
 class ServeWeights:
     """Inference weights extracted from a (LoRA-merged) LlamaForCausalLM, TP-sliced."""
 
-    def __init__(self, model, tp_rank: int = 0, tp_size: int = 1):
+    def __init__(self, model, tp_rank: int = 0, tp_size: int = 1, quantization: Optional[str] = None,
+                 release: bool = False):
+        """``quantization`` "mxfp4": the projections of this rank's slice in 4 bits (``ops/mxfp4.py``), the LM head and the
+        embeddings as they are.  ``release``: the model is the caller's to spend, a layer's 16-bit projections are freed as
+        their quantised form is made."""
+        if quantization not in (None, "mxfp4"):
+            raise ValueError(f"quantization must be None or 'mxfp4', got {quantization!r}")
+        self.quantization = quantization
         cfg: ModelConfig = model.config
         if cfg.arch != "llama":
             raise NotImplementedError("serving supports the Llama family")
@@ -116,14 +129,23 @@ class ServeWeights:
         self.layers: List[LayerW] = []
         with torch.no_grad():
             for L in model.layers:
-                W = L.self_attn.qkv_proj.weight
+                W = _values(L.self_attn.qkv_proj)
                 qkv = torch.cat([W[r * lq:(r + 1) * lq], W[qs + r * lk:qs + (r + 1) * lk],
                                  W[qs + ks + r * lk:qs + ks + (r + 1) * lk]], 0).contiguous()
-                o = L.self_attn.o_proj.weight[:, r * lq:(r + 1) * lq].contiguous()
-                GU = L.mlp.gate_up_proj.weight
+                o = _values(L.self_attn.o_proj)[:, r * lq:(r + 1) * lq].contiguous()
+                GU = _values(L.mlp.gate_up_proj)
                 gu = torch.cat([GU[r * lf:(r + 1) * lf], GU[Fd + r * lf:Fd + (r + 1) * lf]],
                                0).contiguous()
-                dn = L.mlp.down_proj.weight[:, r * lf:(r + 1) * lf].contiguous()
+                dn = _values(L.mlp.down_proj)[:, r * lf:(r + 1) * lf].contiguous()
+                if quantization is not None:
+                    for n, w in (("o", o), ("down", dn), ("q|k|v", qkv)):
+                        if w.shape[1] % 8:
+                            raise ValueError(f"quantization: {n} has {w.shape[1]} inputs a rank, no multiple of 8")
+                    qkv, o, gu, dn = (mxfp4_quantize(w) for w in (qkv, o, gu, dn))
+                    if release:
+                        del W, GU
+                        for lin in (L.self_attn.qkv_proj, L.self_attn.o_proj, L.mlp.gate_up_proj, L.mlp.down_proj):
+                            lin.weight = torch.nn.Parameter(lin.weight.new_empty(0), requires_grad=False)
                 self.layers.append(LayerW(L.input_layernorm.weight, L.post_attention_layernorm.weight,
                                           qkv, o, gu, dn))
         self.embed = model.embed_tokens.weight
@@ -253,6 +275,8 @@ class ModelRunner:
         D = cfg.head_dim
         ml = self.lora if lora_ids is not None else None
         masks = {n: ml.mask(lora_ids, n) for n in (1, 2, 3)} if ml is not None else None
+        if self.w.quantization is not None:
+            return self._layers_mxfp4(h, positions, slots, attn_fn, ml, masks, mark, rotate)
         for i, L in enumerate(self.w.layers):
             if T == 1 and ml is None and row_norm_ok(h, L.ln1, res, L.qkv):
                 qkv, res = row_norm_linear(h, L.ln1, cfg.rms_norm_eps, res, L.qkv)
@@ -296,6 +320,32 @@ class ModelRunner:
             else:
                 act = swiglu(gu)
                 h = self._allreduce(linear_nt(act, L.down))
+                ml.apply(i, "down", act, h, masks, self._allreduce)
+        return h, res
+
+    def _layers_mxfp4(self, h, positions, slots, attn_fn, ml, masks, mark, rotate):
+        """``_layers`` on projections in 4 bits."""
+        eps, res = self.cfg.rms_norm_eps, None
+        for i, L in enumerate(self.w.layers):
+            y, res = rms_norm(h, L.ln1, eps, res)
+            qkv = mxfp4_linear(y, L.qkv)
+            if mark is not None and i == 0:
+                mark.record()
+            if ml is not None:
+                ml.apply(i, "qkv", y, qkv, masks)
+            if rotate:
+                self._rotate_write(qkv, positions, slots, i)
+            o = attn_fn(qkv, i)
+            a = self._allreduce(mxfp4_linear(o, L.o))
+            if ml is not None:
+                ml.apply(i, "o", o, a, masks, self._allreduce)
+            y2, res = rms_norm(a, L.ln2, eps, res)
+            gu = mxfp4_linear(y2, L.gate_up)
+            if ml is not None:
+                ml.apply(i, "gate_up", y2, gu, masks)
+            act = swiglu(gu)
+            h = self._allreduce(mxfp4_linear(act, L.down))
+            if ml is not None:
                 ml.apply(i, "down", act, h, masks, self._allreduce)
         return h, res
 

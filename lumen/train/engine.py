@@ -85,6 +85,10 @@ class ZeroEngine:
                 # weight gathers on their own communicator (own RCCL stream): gradient
                 # reduce-scatters / norm / publish on the default group never queue behind them
                 self.gather_group = dist.new_group(ranks=list(range(W)))
+            from ..models.layers import Linear
+
+            if any(isinstance(m, Linear) and m.qdata is not None for m in model.modules()):
+                raise ValueError("ZeRO-3 partitions 16-bit weights: a base in 4 bits trains at stages 0 - 2")
             self.coordinator = ParamCoordinator(
                 model, env, cfg.stage3_param_persistence_threshold,
                 cfg.stage3_max_live_parameters, cfg.stage3_prefetch_bucket_size,

@@ -19,7 +19,8 @@ import torch
 
 from ..data import (CausalLMCollator, PackedCollator, PrefetchLoader, ShardedSampler,
                     build_dataset, load_tokenizer)
-from ..lora import LoraConfig, apply_lora, print_trainable_parameters, save_adapter
+from ..lora import (LoraConfig, apply_lora, print_trainable_parameters, quantize_base,
+                    save_adapter)
 from ..models import build_model, get_config
 from ..parallel.dist import DistEnv, agree_all, all_reduce_scalar, barrier
 from ..utils.debug import StepProfiler, StepWatchdog, check_finite, maybe_inject_fault
@@ -65,6 +66,7 @@ class TrainArgs:
     log_file: Optional[str] = None
     async_save: bool = True
     fuse_accumulation: bool = True  # equal-size accumulation micro-batches as one forward
+    base_quantization: Optional[str] = None  # "mxfp4": the frozen base in 4 bits (ZeRO 0 - 2)
 
 
 def model_flops_per_token(cfg, seq_len: int, lora: bool = True) -> float:
@@ -96,6 +98,13 @@ class Trainer:
         lcfg = LoraConfig(r=args.lora_r, lora_alpha=args.lora_alpha, lora_dropout=args.lora_dropout,
                           target_modules=args.lora_targets)
         apply_lora(self.model, lcfg)
+        if args.base_quantization:
+            if ds.stage >= 3:
+                raise ValueError("base_quantization: ZeRO-3 partitions 16-bit weights; use stage 0, 1 or 2")
+            if env.device.type == "cuda" and dt == torch.float32:
+                raise ValueError("base_quantization: bf16 or fp16 on the GPU")
+            freed = quantize_base(self.model, args.base_quantization)
+            self.print(f"[lumen] base weights in {args.base_quantization}: {freed / 1e9:.2f} GB freed")
         gc = args.gradient_checkpointing
         gc = gc.lower() if isinstance(gc, str) else gc
         gc = {"true": True, "false": False}.get(gc, gc)
