@@ -274,7 +274,7 @@ def main():
                     help="x token budget while at most max-num-seqs/4 sequences decode (1: off)")
     ap.add_argument("--no-graphs", action="store_true")
     ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"])
-    ap.add_argument("--quantization", default=None, choices=[None, "mxfp4"])
+    ap.add_argument("--quantization", default=None, choices=[None, "mxfp4", "mxfp4_a4"])
     ap.add_argument("--sync-scheduling", action="store_true",
                     help="engine mode: host waits for each step's tokens before the next step")
     ap.add_argument("--tp", type=int, default=1,

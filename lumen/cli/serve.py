@@ -56,9 +56,10 @@ def build_parser():
     ap.add_argument("--no-graphs", action="store_true")
     ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"],
                     help="KV-cache element type (fp8 = e4m3: 2x capacity, half the decode K/V reads)")
-    ap.add_argument("--quantization", default=None, choices=[None, "mxfp4"],
+    ap.add_argument("--quantization", default=None, choices=[None, "mxfp4", "mxfp4_a4"],
                     help="hold the projections in 4-bit floating point, made from the 16-bit "
-                         "weights at start (vLLM's flag; MXFP4: 4.25 bits a weight)")
+                         "weights at start (vLLM's flag; MXFP4: 4.25 bits a weight); mxfp4_a4: "
+                         "their inputs too, for faster prompts")
     ap.add_argument("--enable-prefix-caching", action="store_true",
                     help="share the cached K/V of equal leading prompt blocks across requests "
                          "(vLLM's flag; finished requests' blocks stay cached until evicted)")

@@ -118,24 +118,22 @@ def of_data(data: torch.Tensor, shape: tuple) -> MXFP4:
     return q
 
 
+# (What a call computes on the host is bound by it for few rows, 3 us of the 7 that it takes: hence their form.)
 def _addresses(q: MXFP4) -> tuple:
     """Of its codes and scales."""
     R, K = q.shape
     p = q.data.data_ptr()
-    return p, p + -(-K // PANEL) * R * 64
+    return p, p + (K + 127 >> 7) * R * 64
 
 
-def _rows(x: torch.Tensor, unit: int = 8) -> tuple:
-    """(``x`` [rows, K] itself where its rows are contiguous and at 16-byte addresses, else a copy; its address; values from row to row)."""
-    R, K = x.shape
-    if x.is_neg():
-        x = x.resolve_neg()
+def _rows(x: torch.Tensor, R: int, K: int, unit: int = 8) -> tuple:
+    """(``x`` [R, K] itself where its rows are contiguous and at 16-byte addresses, else a copy; its address; values from row to row)."""
     ld, one = x.stride()
     if R == 1:
-        ld = -(-K // unit) * unit
+        ld = K
     p = x.data_ptr()
-    if (one != 1 and K > 1) or p % 16 or ld % unit or not K <= ld <= MAX_LD:
-        x = x.clone(memory_format=torch.contiguous_format)
+    if one != 1 or p & 15 or ld % unit or not K <= ld <= MAX_LD or x.is_neg():
+        x = x.resolve_neg().clone(memory_format=torch.contiguous_format)
         p, ld = x.data_ptr(), K
     return x, p, ld
 
@@ -171,7 +169,7 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4:
     dev, dt = x.device, DT[x.dtype]
     q = of_data(torch.empty(_nbytes(R, K), dtype=torch.uint8, device=dev), (R, K))
     if R:
-        x, p, ld = _rows(x.detach() if x.requires_grad else x, 8 if dt else 4)
+        x, p, ld = _rows(x.detach() if x.requires_grad else x, R, K, 8 if dt else 4)
         _launch("sm_mx_quantize", dev, dt, p, ld, *_addresses(q), R, K)
     return q
 
@@ -280,6 +278,8 @@ def _check(name: str, K: int, device, w, bias: Optional[torch.Tensor], dtype: to
         raise ValueError(f"{name}: rows of {K} values against a weight of {w.shape[1]}")
     if w.data.device != device:
         raise ValueError(f"{name}: rows on {device}, weight on {w.device}")
+    if K > MAX_LD:
+        raise ValueError(f"{name}: rows of {K} values (at most {MAX_LD})")
     if bias is not None:
         if bias.dim() != 1 or bias.shape[0] != w.shape[0] or bias.dtype != dtype or bias.device != device:
             raise ValueError(f"{name}: the bias is not [{w.shape[0]}] values of {dtype} on {device}")
@@ -295,11 +295,12 @@ def linear_rows(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) 
         return (y if bias is None else y + bias.float()).to(x.dtype)
     y = torch.empty((M, N), dtype=x.dtype, device=x.device)
     if M and N:
-        x, p, ld = _rows(x)
+        x, p, ld = _rows(x, M, K)
         if bias is not None:
             bias = bias.contiguous()
         tiles, m, n = _linear_form(M, N, K)
-        _launch("sm_mx_linear" if tiles else "sm_mx_rows", y.device, DT[x.dtype], p, ld, *_addresses(w), 0 if bias is None else bias.data_ptr(),
+        wc, ws = _addresses(w)
+        _launch("sm_mx_linear" if tiles else "sm_mx_rows", y.device, DT[y.dtype], p, ld, wc, ws, 0 if bias is None else bias.data_ptr(),
                 y.data_ptr(), M, N, K, m, n)
     return y
 
@@ -314,7 +315,7 @@ def input_grad(dy: torch.Tensor, w: MXFP4) -> torch.Tensor:
     dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
     if N % 8:                                      # (rows at 16-byte addresses, zeros behind them)
         dy = F.pad(dy, (0, -N % 8))
-    dy, p, ld = _rows(dy)
+    dy, p, ld = _rows(dy, *dy.shape)
     tiles, m, wn = _grad_form(M, N, K)
     args = (DT[dy.dtype], p, ld, *_addresses(w), dx.data_ptr(), M, N, K, m)
     if tiles:
@@ -357,13 +358,18 @@ def mxfp4_linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None)
     sums, one rounding to x's type (bf16 or fp16; on the CPU fp32 too).  Differentiable in x, not in the weight or the bias."""
     if x.dim() < 1 or x.dtype not in (HALF if x.is_cuda else DT):
         raise ValueError("mxfp4_linear: rows [..., K] of bf16 or fp16")
-    K = x.shape[-1]
-    _check("mxfp4_linear", K, x.device, w, bias, x.dtype)
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    sh = x.shape
+    _check("mxfp4_linear", sh[-1], x.device, w, bias, x.dtype)
+    x2 = x if len(sh) == 2 else x.reshape(-1, sh[-1])
     if x2.shape[0] > MAX_ROWS:
         raise ValueError(f"mxfp4_linear: {x2.shape[0]} rows (at most {MAX_ROWS})")
-    y = _Linear.apply(x2, w, bias) if x.requires_grad and torch.is_grad_enabled() else linear_rows(x2, w, bias)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
+    if x.requires_grad and torch.is_grad_enabled():
+        if w.shape[0] > MAX_LD:
+            raise ValueError(f"mxfp4_linear: {w.shape[0]} columns with a gradient (at most {MAX_LD})")
+        y = _Linear.apply(x2, w, bias)
+    else:
+        y = linear_rows(x2, w, bias)
+    return y if len(sh) == 2 else y.view(*sh[:-1], w.shape[0])
 
 
 def mxfp4_matmul(a: MXFP4, b: MXFP4, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:

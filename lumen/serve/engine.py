@@ -23,7 +23,8 @@ import torch.distributed as dist
 
 from ..models import build_model, get_config
 from .block_manager import BlockManager
-from .model_runner import ModelRunner, ServeWeights, StepInput, kv_bytes_per_token
+from .model_runner import (QUANTIZATIONS, ModelRunner, ServeWeights, StepInput,
+                           kv_bytes_per_token)
 from .scheduler import Batch, Scheduler, SchedulerConfig
 from .sequence import SamplingParams, Sequence, Status
 
@@ -65,8 +66,9 @@ class EngineConfig:
     # KV-cache element type: "auto" = model dtype; "fp8" = e4m3 (vLLM --kv-cache-dtype fp8):
     # twice the cache capacity and half the K/V bytes per decode step, at fp8 K/V precision
     kv_cache_dtype: str = "auto"
-    # projections in 4-bit floating point ("mxfp4", made from the 16-bit weights at start; vLLM --quantization): 4.25 bits
-    # a weight instead of 16.  LM head, embeddings, norms and adapters keep the model dtype
+    # projections in 4-bit floating point ("mxfp4", made from the 16-bit weights at start; vLLM --quantization; 4.25 bits
+    # a weight instead of 16; "mxfp4_a4": the projections' inputs too, on the 4-bit matrix instructions: faster prompts, less
+    # exact).  LM head, embeddings, norms and adapters keep the model dtype
     quantization: Optional[str] = None
     # automatic prefix caching (vLLM --enable-prefix-caching): prompts share the cached K/V of
     # equal leading full blocks; finished sequences' blocks stay cached until evicted
@@ -145,8 +147,8 @@ class LLMEngine:
 
             load_tuned_gemms()  # tuned hipBLASLt algorithms for the prefill/decode GEMM shapes
         dt = _DT[cfg.dtype] if dev.type == "cuda" else torch.float32
-        if cfg.quantization not in (None, "mxfp4"):
-            raise ValueError(f"quantization must be None or 'mxfp4', got {cfg.quantization!r}")
+        if cfg.quantization not in QUANTIZATIONS:
+            raise ValueError(f"quantization must be one of {QUANTIZATIONS}, got {cfg.quantization!r}")
         if cfg.quantization and dev.type == "cuda" and dt == torch.float32:
             raise ValueError("quantization: dtype bf16 or fp16 on the GPU")
         own_model = model is None

@@ -37,7 +37,7 @@ from ..ops.attention import (flash_attention_fresh, flash_attention_paged, paged
                              rope_write_kv)
 from ..ops.gemm import decoded_rows, linear_nt, row_norm_linear, row_norm_ok, swiglu_linear_nt
 from ..ops.moe import MID_MAX_M, THIN_ACT_MAX_M, mid_act, mid_act_ok, thin_act, thin_act_ok, tile_act, tile_act_ok
-from ..ops.mxfp4 import mxfp4_linear, mxfp4_quantize
+from ..ops.mxfp4 import mxfp4_linear, mxfp4_matmul, mxfp4_quantize
 from ..ops.norm import rms_norm
 from ..ops.rope import rope_tables
 
@@ -97,9 +97,17 @@ class LayerW:
     down: torch.Tensor
 
 
+QUANTIZATIONS = (None, "mxfp4", "mxfp4_a4")
+
+
 def _values(lin) -> torch.Tensor:
     """A projection's weight, of a 4-bit base its values."""
     return lin.weight if lin.qdata is None else lin.qweight.dequantize(lin.weight.dtype)
+
+
+def _linear_a4(x, w):
+    """x @ w^T with both in 4 bits."""
+    return mxfp4_matmul(mxfp4_quantize(x), w, out_dtype=x.dtype)
 
 
 class ServeWeights:
@@ -108,10 +116,10 @@ class ServeWeights:
     def __init__(self, model, tp_rank: int = 0, tp_size: int = 1, quantization: Optional[str] = None,
                  release: bool = False):
         """``quantization`` "mxfp4": the projections of this rank's slice in 4 bits (``ops/mxfp4.py``), the LM head and the
-        embeddings as they are.  ``release``: the model is the caller's to spend, a layer's 16-bit projections are freed as
+        embeddings as they are; "mxfp4_a4": their inputs too, quantised row by row as they come.  ``release``: the model is the caller's to spend, a layer's 16-bit projections are freed as
         their quantised form is made."""
-        if quantization not in (None, "mxfp4"):
-            raise ValueError(f"quantization must be None or 'mxfp4', got {quantization!r}")
+        if quantization not in QUANTIZATIONS:
+            raise ValueError(f"quantization must be one of {QUANTIZATIONS}, got {quantization!r}")
         self.quantization = quantization
         cfg: ModelConfig = model.config
         if cfg.arch != "llama":
@@ -326,9 +334,10 @@ class ModelRunner:
     def _layers_mxfp4(self, h, positions, slots, attn_fn, ml, masks, mark, rotate):
         """``_layers`` on projections in 4 bits."""
         eps, res = self.cfg.rms_norm_eps, None
+        linear = mxfp4_linear if self.w.quantization == "mxfp4" else _linear_a4
         for i, L in enumerate(self.w.layers):
             y, res = rms_norm(h, L.ln1, eps, res)
-            qkv = mxfp4_linear(y, L.qkv)
+            qkv = linear(y, L.qkv)
             if mark is not None and i == 0:
                 mark.record()
             if ml is not None:
@@ -336,15 +345,15 @@ class ModelRunner:
             if rotate:
                 self._rotate_write(qkv, positions, slots, i)
             o = attn_fn(qkv, i)
-            a = self._allreduce(mxfp4_linear(o, L.o))
+            a = self._allreduce(linear(o, L.o))
             if ml is not None:
                 ml.apply(i, "o", o, a, masks, self._allreduce)
             y2, res = rms_norm(a, L.ln2, eps, res)
-            gu = mxfp4_linear(y2, L.gate_up)
+            gu = linear(y2, L.gate_up)
             if ml is not None:
                 ml.apply(i, "gate_up", y2, gu, masks)
             act = swiglu(gu)
-            h = self._allreduce(mxfp4_linear(act, L.down))
+            h = self._allreduce(linear(act, L.down))
             if ml is not None:
                 ml.apply(i, "down", act, h, masks, self._allreduce)
         return h, res

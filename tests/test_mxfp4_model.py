@@ -116,6 +116,24 @@ def test_engine_answers_as_with_the_quantised_values():
     assert answers(engine(m)) == want
 
 
+def test_engine_with_inputs_in_4_bits_too():
+    """Against full forwards of the model with the quantised values whose projections see quantised rows."""
+    _, plain = pair(lora=False, seed=1)
+    for n, lin in plain.named_modules():
+        if isinstance(lin, Linear) and not n.endswith("lm_head"):
+            lin.register_forward_pre_hook(lambda mod, a: (mxfp4_quantize(a[0]).dequantize(torch.float32),))
+    plain.eval()
+    torch.manual_seed(1)
+    eng = engine(build_model("tiny-llama-gqa", dtype=torch.float32, init="random", seed=1), quantization="mxfp4_a4")
+    got = answers(eng)
+    for p, out in zip(([5, 9, 33, 7] * 6, [42, 43], list(range(3, 30))), got):
+        ids = list(p)
+        for tok in out:
+            with torch.no_grad():
+                assert int(plain(torch.tensor([ids])).view(len(ids), -1)[-1].argmax()) == tok
+            ids.append(tok)
+
+
 def test_engine_frees_the_model_that_it_builds():
     eng = engine(None, quantization="mxfp4", init="random")
     assert type(eng.weights.layers[0].down) is MXFP4 and len(answers(eng)) == 3
