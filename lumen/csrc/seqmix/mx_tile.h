@@ -50,16 +50,16 @@ __device__ __forceinline__ void put(const TileArgs& a, int m, int n, bool two, c
 // the results of a wave, whose fragments of w stand for columns as tile::colperm says
 template <typename T, int NI, int MJ>
 __device__ __forceinline__ void put_all(const TileArgs& a, f32x4 (&acc)[NI][MJ], int m0, int n0) {
+  static_assert(NI % 2 == 0, "columns in pairs of fragments");
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
 #pragma unroll
   for (int j = 0; j < MJ; ++j) {
     const int m = m0 + 16 * j + lr;
 #pragma unroll
     for (int i = 0; i < NI; i += 2) {
-      const bool two = i + 1 < NI;
       hold<kNamed<NI, MJ>>(acc[i][j]);
-      if (two) hold<kNamed<NI, MJ>>(acc[i + 1 < NI ? i + 1 : i][j]);
-      if (m < a.M) put<T>(a, m, n0 + 16 * i + (two ? 8 : 4) * lg, two, acc[i][j], acc[i + 1 < NI ? i + 1 : i][j]);
+      hold<kNamed<NI, MJ>>(acc[i + 1][j]);
+      if (m < a.M) put<T>(a, m, n0 + 16 * i + 8 * lg, true, acc[i][j], acc[i + 1][j]);
     }
   }
 }

@@ -71,7 +71,7 @@ class Linear(nn.Module):
                                    requires_grad=False)
         self.bias = (nn.Parameter(torch.zeros(out_features, dtype=dtype, device=device),
                                   requires_grad=False) if bias else None)
-        self.register_buffer("qdata", None, persistent=False)  # the weight in MXFP4 (quantize_base)
+        self.register_buffer("qdata", None)  # the weight in MXFP4 (quantize_base)
         self.seg_sizes = list(seg_sizes) if seg_sizes else [out_features]
         self.seg_names = list(seg_names) if seg_names else ["proj"]
         self.lora: Optional[LoRAAdapter] = None

@@ -84,6 +84,17 @@ def test_gradient_of_the_rows():
     assert abs(float(fd - (dx.double() * d.double()).sum())) <= float(size) * (64 + 9) * 2.0 ** -23
 
 
+def test_the_gradient_can_be_differentiated():
+    w = mxfp4_quantize(torch.randn(9, 64))
+    W = ref.values(w)
+    x = torch.randn(4, 64, requires_grad=True)
+    dy = torch.randn(4, 9, requires_grad=True)
+    (dx,) = torch.autograd.grad(mxfp4_linear(x, w), x, dy, create_graph=True)
+    g = torch.randn(4, 64)
+    (ddy,) = torch.autograd.grad(dx, dy, g)
+    ref.close(ddy, g.double() @ W.t(), g.double().abs() @ W.abs().t(), 64, torch.float32)
+
+
 def test_empty():
     w = mxfp4_quantize(torch.randn(4, 64))
     assert mxfp4_linear(torch.randn(0, 64), w).shape == (0, 4)
@@ -128,3 +139,8 @@ def test_refusals():
     refused(mxfp4_matmul, w, w, out_dtype=torch.float64)
     refused(mxfp4_matmul, w, w, bias=torch.zeros(4))      # fp32 bias, bf16 result
     refused(mxfp4_matmul, w, mxfp4_quantize(torch.randn(4, 96)))
+    long = MXFP4(u8(1, 1 << 22), u8(1, 1 << 18))          # 2^23 values a row: to quantise and back, not to multiply
+    assert long.dequantize().shape == (1, 1 << 23)
+    refused(mxfp4_linear, torch.zeros(1, 1 << 23), long)
+    refused(mxfp4_matmul, long, long)
+    refused(MXFP4, u8(1, (1 << 22) + 4), u8(1, (1 << 18) + 1))

@@ -339,3 +339,72 @@ def test_empty_on_the_gpu():
     x = randn(1, 3, 64).bfloat16().requires_grad_()
     (dx,) = torch.autograd.grad(mxfp4_linear(x, e).sum(), x)
     assert mxfp4_matmul(q, e).shape == (16, 0) and int(dx.abs().sum()) == 0
+
+
+def test_results_past_32_bits():
+    """36000 x 65536 values and results: the last rows equal those of a call that has only them."""
+    M, N, K = 36000, 65536, 64
+    q, _ = weight(3, N, K)
+    x = randn(1, M, K).bfloat16()
+    W, X = ref.values(q), x[-40:].double().cpu()
+    y = mxfp4_linear(x, q)
+    ref.close(y[-40:], X @ W.t(), X.abs() @ W.abs().t(), K, torch.bfloat16)
+    a = mxfp4_quantize(y)
+    assert torch.equal(a.codes[-40:], mxfp4_quantize(y[-40:]).codes) and torch.equal(a.scales[-40:], mxfp4_quantize(y[-40:]).scales)
+    back = mxfp4_dequantize(a)
+    assert torch.equal(back[-40:], mxfp4_dequantize(mxfp4_quantize(y[-40:])))
+    del back
+    t, _ = weight(5, K, N)                                # rows of y against 64 rows, and their gradient as large as y
+    dx = mx.input_grad(x, t)
+    V = ref.values(t)
+    ref.close(dx[-40:], X @ V, X.abs() @ V.abs(), K, torch.bfloat16)
+    del dx
+    z = mxfp4_matmul(mxfp4_quantize(x), q)
+    A = ref.values(mxfp4_quantize(x[-40:]))
+    ref.close(z[-40:], A @ W.t(), A.abs() @ W.abs().t(), K, torch.bfloat16)
+
+
+@pytest.mark.parametrize("M", [1, 20, 70])
+def test_the_longest_rows(M):
+    """2^22 values a row, 65 of them not zero."""
+    K = mx.MAX_LD
+    at = torch.cat((torch.randint(0, K, (64,), generator=torch.Generator().manual_seed(M)), torch.tensor([K - 1]))).unique().cuda()
+    x = torch.zeros(M, K, device="cuda", dtype=torch.bfloat16)
+    x[:, at] = randn(M, M, len(at)).bfloat16()
+    w = torch.zeros(24, K, device="cuda", dtype=torch.bfloat16)
+    w[:, at] = randn(7, 24, len(at)).bfloat16()
+    q = mxfp4_quantize(w)
+    W = mxfp4_dequantize(q)[:, at].double().cpu()
+    X = x[:, at].double().cpu()
+    ref.close(mxfp4_linear(x, q), X @ W.t(), X.abs() @ W.abs().t(), 65, torch.bfloat16)
+    a = mxfp4_quantize(x)
+    A = mxfp4_dequantize(a)[:, at].double().cpu()
+    ref.close(mxfp4_matmul(a, q), A @ W.t(), A.abs() @ W.abs().t(), 65, torch.bfloat16)
+    g = mx.input_grad(randn(3, M, 24).bfloat16(), q)
+    G = randn(3, M, 24).bfloat16().double().cpu()
+    ref.close(g[:, at], G @ W, G.abs() @ W.abs(), 24, torch.bfloat16)
+
+
+def test_the_gradient_can_be_differentiated_on_the_gpu():
+    q, W = weight(1, 52, 96)
+    x = randn(1, 20, 96).bfloat16().requires_grad_()
+    dy = randn(2, 20, 52).bfloat16().requires_grad_()
+    (dx,) = torch.autograd.grad(mxfp4_linear(x, q), x, dy, create_graph=True)
+    g = randn(3, 20, 96).bfloat16()
+    (ddy,) = torch.autograd.grad(dx, dy, g)
+    G = g.double().cpu()
+    ref.close(ddy, G @ W.t(), G.abs() @ W.abs().t(), 96, torch.bfloat16)
+
+
+def test_a_bias_between_other_values():
+    """A bias that is every second value of a buffer, another that starts at an odd address."""
+    q, W = weight(2, 50, 96)
+    x = randn(1, 5, 96).bfloat16()
+    X = x.double().cpu()
+    buf = randn(4, 101).bfloat16()
+    for b in (buf[::2][:50], buf[1:51]):
+        B = b.double().cpu()
+        ref.close(mxfp4_linear(x, q, b), X @ W.t() + B, X.abs() @ W.abs().t() + B.abs(), 97, torch.bfloat16)
+        a = mxfp4_quantize(x)
+        A = ref.values(a)
+        ref.close(mxfp4_matmul(a, q, b), A @ W.t() + B, A.abs() @ W.abs().t() + B.abs(), 97, torch.bfloat16)

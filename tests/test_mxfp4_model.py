@@ -88,6 +88,20 @@ def test_quantised_bases_move_copy_and_come_back():
     assert torch.equal(lin.qweight.codes, codes)          # quantised values stay what they are
 
 
+def test_state_dict_holds_the_base():
+    m, _ = pair(lora=False, seed=3)
+    other, _ = pair(lora=False, seed=4)
+    other.load_state_dict(m.state_dict())
+    for a, b in zip(m.modules(), other.modules()):
+        if isinstance(a, Linear) and a.qdata is not None:
+            assert torch.equal(a.qdata, b.qdata)
+    whole = build_model("tiny-llama-gqa", dtype=torch.float32, init="random", seed=5)
+    with pytest.raises(RuntimeError):
+        whole.load_state_dict(m.state_dict())
+    with pytest.raises(RuntimeError):
+        m.load_state_dict(whole.state_dict())
+
+
 def engine(model, **kw):
     from lumen.serve.engine import EngineConfig, LLMEngine
 
@@ -132,6 +146,32 @@ def test_engine_with_inputs_in_4_bits_too():
             with torch.no_grad():
                 assert int(plain(torch.tensor([ids])).view(len(ids), -1)[-1].argmax()) == tok
             ids.append(tok)
+
+
+def test_engine_adds_adapters_to_projections_in_4_bits(tmp_path):
+    """A batch of plain and adapted requests against engines whose weights are the quantised values, adapters merged."""
+    from lumen.lora import load_adapter, save_adapter
+    from lumen.serve.sequence import SamplingParams
+
+    m, plain = pair(lora=False, seed=1)
+    adapted = copy.deepcopy(plain)
+    apply_lora(adapted, LoraConfig(r=4, lora_dropout=0.0, target_modules=["q_proj", "v_proj", "o_proj", "up_proj", "down_proj"]))
+    with torch.no_grad():
+        for p in adapted.parameters():
+            if p.requires_grad:
+                p.normal_(0, 0.1)
+    save_adapter(adapted, str(tmp_path / "a"), "tiny-llama-gqa")
+    eng = engine(m, quantization="mxfp4", lora_modules={"a": str(tmp_path / "a")}, max_loras=2)
+    params = dict(max_tokens=8, temperature=0.0, ignore_eos=True)
+    prompts = ([5, 9, 33, 7] * 6, [42, 43], list(range(3, 30)))
+    which = (None, "a", "a")
+    seqs = [eng.add_request(p, SamplingParams(**params), lora=w) for p, w in zip(prompts, which)]
+    while eng.has_work:
+        eng.step()
+    load_adapter(plain_a := copy.deepcopy(plain), str(tmp_path / "a"))
+    merge_lora(plain_a)
+    for p, w, s in zip(prompts, which, seqs):
+        assert s.output_ids == answers(engine(plain if w is None else plain_a))[prompts.index(p)]
 
 
 def test_engine_frees_the_model_that_it_builds():

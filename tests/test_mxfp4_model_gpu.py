@@ -124,3 +124,42 @@ def test_engine_logits(name, graphs):
             with torch.no_grad():
                 ref = plain(ids).float().view(pos + 1, -1)[-1]
             assert (logits[i] - ref).norm() <= 3e-2 * ref.norm()
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_engine_with_inputs_in_4_bits_too(graphs):
+    """Decode steps against the full forward of the model whose projections see quantised rows.  Both round in 16 bits before they
+    quantise, and a value within that rounding v 2^-8 of a tie may take the other code.  v is some four steps at most, so two
+    hundredths of the values do, a step each: 0.02 step^2 against the step^2 / 12 of quantisation itself, half its norm.  Allowed
+    is the whole distance that quantising the rows makes, and the 3 % of 16-bit arithmetic."""
+    from lumen.ops.mxfp4 import mxfp4_quantize
+    from lumen.serve.engine import EngineConfig, LLMEngine
+    from lumen.serve.sequence import SamplingParams
+
+    m, plain = pair("tiny-llama-gqa", torch.bfloat16, lora=False)
+    m.eval(), plain.eval()
+    rows = copy.deepcopy(plain)
+    for n, lin in rows.named_modules():
+        if isinstance(lin, Linear) and not n.endswith("lm_head"):
+            lin.register_forward_pre_hook(
+                lambda mod, a: (mxfp4_quantize(a[0].reshape(-1, a[0].shape[-1])).dequantize(a[0].dtype).view(a[0].shape),))
+    eng = LLMEngine(EngineConfig(model="tiny-llama-gqa", device="cuda", max_model_len=256, block_size=16, num_blocks=128, use_graphs=graphs,
+                                 quantization="mxfp4_a4"), model=m)
+    prompts = [list(range(10, 40)), [7, 8, 9] * 20, [42]]
+    seqs = [eng.add_request(p, SamplingParams(max_tokens=6, temperature=0, ignore_eos=True)) for p in prompts]
+    got, orig = [], eng.runner.decode
+
+    def spy(inp):
+        out = orig(inp)
+        got.append((inp.positions.cpu().tolist(), out.float().clone()))
+        return out
+    eng.runner.decode = spy
+    while eng.has_work:
+        eng.step()
+    assert got
+    for positions, logits in got:
+        for i, (s, pos) in enumerate(zip(seqs, positions)):
+            ids = torch.tensor([s.all_ids[:pos + 1]], device="cuda")
+            with torch.no_grad():
+                with_q, without = (mod(ids).float().view(pos + 1, -1)[-1] for mod in (rows, plain))
+            assert (logits[i] - with_q).norm() <= (with_q - without).norm() + 3e-2 * without.norm()
