@@ -2,8 +2,8 @@
 //
 // Every function here only checks arguments, picks the dtype code and the current HIP stream,
 // and calls an `extern "C"` launcher from kernels/*.hip.  Allocation and shape logic live in
-// lumen/ops/*.py so this translation unit (the only one that includes the heavy torch headers)
-// rarely changes.
+// lumen/ops/*.py so this translation unit (with mx_calls.cpp, the products with 4-bit weights, the only one that includes the
+// heavy torch headers) rarely changes.
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
@@ -1080,8 +1080,11 @@ void car_allreduce(const std::vector<int64_t>& data, const std::vector<int64_t>&
         "car_allreduce");
 }
 
+void bind_mx_calls(pybind11::module_&);      // mx_calls.cpp
+
 PYBIND11_MODULE(_C, m) {
   m.doc() = "lumen native ops for MI355X (gfx950)";
+  bind_mx_calls(m);
   m.def("rmsnorm_fwd", &rmsnorm_fwd);
   m.def("lora3_down", &lora3_down, py::arg("x"), py::arg("ldx"), py::arg("A"), py::arg("Z"),
         py::arg("ldz"), py::arg("T"), py::arg("K"), py::arg("R"), py::arg("alpha"), py::arg("seed"),

@@ -80,11 +80,16 @@ def _torch_flags():
     return cflags, ldflags
 
 
+def _bindings() -> list:
+    """Host code that needs the torch headers."""
+    return [os.path.join(HERE, "binding.cpp"), os.path.join(HERE, "mx_calls.cpp")]
+
+
 def sources() -> list:
     """Every source the extension is built from (kernels, headers, host code, binding)."""
     return sorted(glob.glob(os.path.join(HERE, "kernels", "*.hip"))
                   + glob.glob(os.path.join(HERE, "kernels", "*.h"))
-                  + [os.path.join(HERE, "cpu", "cpu_adam.cpp"), os.path.join(HERE, "binding.cpp")])
+                  + [os.path.join(HERE, "cpu", "cpu_adam.cpp"), *_bindings()])
 
 
 def source_digest() -> dict:
@@ -202,14 +207,14 @@ def _build_locked(jobs, force, verbose, build_dir, out) -> str:
     cmd = ["g++", "-O3", "-fPIC", "-std=c++17", "-fopenmp", "-c", cpu_src, "-o", cpu_obj]
     if force or _newer([cpu_src], cpu_obj) or not _same_command(cmd, cpu_obj):
         jobs_list.append(cmd)
-    bind_src = os.path.join(HERE, "binding.cpp")
-    bind_obj = os.path.join(build_dir, "binding.o")
-    objs.append(bind_obj)
     cflags, ldflags = _torch_flags()
-    # host-only translation unit: plain g++ against the HIP host API headers
-    cmd = ["g++", "-O2", "-fPIC", "-std=c++17", f"-I{ROCM}/include", *cflags, "-c", bind_src, "-o", bind_obj]
-    if force or _newer([bind_src], bind_obj) or not _same_command(cmd, bind_obj):
-        jobs_list.append(cmd)
+    # host-only translation units: plain g++ against the HIP host API headers
+    for src in _bindings():
+        obj = os.path.join(build_dir, os.path.splitext(os.path.basename(src))[0] + ".o")
+        objs.append(obj)
+        cmd = ["g++", "-O2", "-fPIC", "-std=c++17", f"-I{ROCM}/include", *cflags, "-c", src, "-o", obj]
+        if force or _newer([src], obj) or not _same_command(cmd, obj):
+            jobs_list.append(cmd)
     if jobs_list:
         with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
             for cmd, (dt, _) in zip(jobs_list, ex.map(_run, jobs_list)):

@@ -9,11 +9,12 @@ code, 6 beyond it).  Two share a byte, the first in its low half.  A block with 
     y = mxfp4_matmul(mxfp4_quantize(x), w)     # both operands in 4 bits, on the scaled matrix instructions
     mxfp4_dequantize(w, torch.bfloat16)
 
-On the GPU these are HIP kernels (``csrc/seqmix/mxfp4.hip``, ``mx_*.hip``); CPU tensors take the torch path below.  The
+On the GPU these are HIP kernels (``csrc/seqmix/mxfp4.hip``, ``mx_*.hip``; ``csrc/mx_calls.cpp`` calls them); CPU tensors take the torch path below.  The
 weight holds no gradient: it is the frozen base of adapters, or served.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 from typing import Optional
 
@@ -21,7 +22,8 @@ import torch
 import torch.nn.functional as F
 
 from . import _seqmix
-from ._seqmix import DT, use_seqmix
+from ._native import native, native_error
+from ._seqmix import DT
 
 BLOCK = 32                # values that share a scale
 PANEL = 128               # values of a row that lie together (csrc/seqmix/mxfp4.hip)
@@ -118,42 +120,23 @@ def of_data(data: torch.Tensor, shape: tuple) -> MXFP4:
     return q
 
 
-# (What a call computes on the host is bound by it for few rows, 3 us of the 7 that it takes: hence their form.)
-def _addresses(q: MXFP4) -> tuple:
-    """Of its codes and scales."""
-    R, K = q.shape
-    p = q.data.data_ptr()
-    return p, p + (K + 127 >> 7) * R * 64
+# what csrc/mx_calls.cpp launches, in its order
+_LAUNCHERS = ("sm_mx_quantize", "sm_mx_dequantize", "sm_mx_linear", "sm_mx_rows", "sm_mx_grad", "sm_mx_rows_grad", "sm_mx_matmul",
+              "sm_mx_rows_matmul")
+_calls = None
 
 
-def _rows(x: torch.Tensor, R: int, K: int, unit: int = 8) -> tuple:
-    """(``x`` [R, K] itself where its rows are contiguous and at 16-byte addresses, else a copy; its address; values from row to row)."""
-    ld, one = x.stride()
-    if R == 1:
-        ld = K
-    p = x.data_ptr()
-    if one != 1 or p & 15 or ld % unit or not K <= ld <= MAX_LD or x.is_neg():
-        x = x.resolve_neg().clone(memory_format=torch.contiguous_format)
-        p, ld = x.data_ptr(), K
-    return x, p, ld
-
-
-_fns: dict = {}
-
-
-def _launch(name: str, device: torch.device, *args) -> None:
-    """The library's ``name`` on the current stream of ``device``, which becomes the current device for it."""
-    fn = _fns.get(name)
-    if fn is None:
-        fn = _fns[name] = getattr(_seqmix._load(), name)
-    i = device.index
-    if i == torch._C._cuda_getDevice():            # (nearly always: as little host time as can be)
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
-    else:
-        with torch.cuda.device(i):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
-    if rc:
-        raise RuntimeError(f"{name}: HIP error {rc}")
+def _native_calls():
+    """The extension's calls, with the kernel library's launchers handed to them once."""
+    global _calls
+    if _calls is None:
+        lib, C = _seqmix._load(), native()
+        if lib is None or C is None:
+            raise RuntimeError(f"lumen kernels are not available ({_seqmix.seqmix_error() or native_error()!r}); build them with "
+                               "`python -m lumen.csrc.build`")
+        C.mx_launchers([ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _LAUNCHERS])
+        _calls = C
+    return _calls
 
 
 # ---- the format -------------------------------------------------------------------------------------
@@ -164,14 +147,9 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4:
     R, K = x.shape
     if K % 8 or not 0 < K <= MAX_K or R > MAX_ROWS:
         raise ValueError(f"mxfp4_quantize: {R} rows of {K} values (at most {MAX_ROWS}; a multiple of 8, at most {MAX_K})")
-    if not use_seqmix(x):
+    if not x.is_cuda:
         return MXFP4(*_encode(x.detach()))
-    dev, dt = x.device, DT[x.dtype]
-    q = of_data(torch.empty(_nbytes(R, K), dtype=torch.uint8, device=dev), (R, K))
-    if R:
-        x, p, ld = _rows(x.detach() if x.requires_grad else x, R, K, 8 if dt else 4)
-        _launch("sm_mx_quantize", dev, dt, p, ld, *_addresses(q), R, K)
-    return q
+    return of_data((_calls or _native_calls()).mx_quantize(x), (R, K))
 
 
 def mxfp4_dequantize(q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -179,13 +157,9 @@ def mxfp4_dequantize(q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
     its largest number).  What lies beyond ``dtype``'s largest number becomes infinite."""
     if dtype not in DT:
         raise ValueError("mxfp4_dequantize: fp32, bf16 or fp16")
-    if not use_seqmix(q.data):
+    if not q.data.is_cuda:
         return _decode(q.codes, q.scales).to(dtype)
-    R, K = q.shape
-    y = torch.empty(R, K, dtype=dtype, device=q.data.device)
-    if R:
-        _launch("sm_mx_dequantize", y.device, DT[dtype], *_addresses(q), y.data_ptr(), R, K)
-    return y
+    return (_calls or _native_calls()).mx_dequantize(q.data, *q.shape, dtype)
 
 
 _VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
@@ -288,69 +262,20 @@ def _check(name: str, K: int, device, w, bias: Optional[torch.Tensor], dtype: to
 
 
 def linear_rows(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``mxfp4_linear`` of checked rows [M, K], without autograd."""
+    """``mxfp4_linear`` of checked rows [M, K], on the GPU without autograd."""
     (M, K), N = x.shape, w.shape[0]
-    if not use_seqmix(x):
+    if not x.is_cuda:
         y = x.float() @ _decode(w.codes, w.scales).to(x.dtype).float().t()
         return (y if bias is None else y + bias.float()).to(x.dtype)
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    if M and N:
-        x, p, ld = _rows(x, M, K)
-        if bias is not None:
-            bias = bias.contiguous()
-        tiles, m, n = _linear_form(M, N, K)
-        wc, ws = _addresses(w)
-        _launch("sm_mx_linear" if tiles else "sm_mx_rows", y.device, DT[y.dtype], p, ld, wc, ws, 0 if bias is None else bias.data_ptr(),
-                y.data_ptr(), M, N, K, m, n)
-    return y
+    return (_calls or _native_calls()).mx_linear(x, w.data, N, bias, *_linear_form(M, N, K))
 
 
 def input_grad(dy: torch.Tensor, w: MXFP4) -> torch.Tensor:
     """dx [M, K] = dy [M, N] times the weight's values in dy's type."""
     (M, N), K = dy.shape, w.shape[1]
-    if not use_seqmix(dy):
+    if not dy.is_cuda:
         return (dy.float() @ _decode(w.codes, w.scales).to(dy.dtype).float()).to(dy.dtype)
-    if not (M and N):
-        return torch.zeros(M, K, dtype=dy.dtype, device=dy.device)
-    dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
-    if N % 8:                                      # (rows at 16-byte addresses, zeros behind them)
-        dy = F.pad(dy, (0, -N % 8))
-    dy, p, ld = _rows(dy, *dy.shape)
-    tiles, m, wn = _grad_form(M, N, K)
-    args = (DT[dy.dtype], p, ld, *_addresses(w), dx.data_ptr(), M, N, K, m)
-    if tiles:
-        _launch("sm_mx_grad", dx.device, *args, wn)
-    else:
-        _launch("sm_mx_rows_grad", dx.device, *args)
-    return dx
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, bias):
-        ctx.save_for_backward(w.data)
-        ctx.shape = w.shape
-        return linear_rows(x, w, bias)
-
-    @staticmethod
-    def backward(ctx, dy):
-        w = of_data(*ctx.saved_tensors, ctx.shape)
-        twice = dy.requires_grad and torch.is_grad_enabled()
-        return _InputGrad.apply(dy, w) if twice else input_grad(dy, w), None, None
-
-
-class _InputGrad(torch.autograd.Function):
-    """The gradient, where it is to be differentiated once more."""
-
-    @staticmethod
-    def forward(ctx, dy, w):
-        ctx.save_for_backward(w.data)
-        ctx.shape = w.shape
-        return input_grad(dy, w)
-
-    @staticmethod
-    def backward(ctx, g):
-        return mxfp4_linear(g, of_data(*ctx.saved_tensors, ctx.shape)), None
+    return (_calls or _native_calls()).mx_grad(dy, w.data, K, *_grad_form(M, N, K))
 
 
 def mxfp4_linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -363,10 +288,11 @@ def mxfp4_linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None)
     x2 = x if len(sh) == 2 else x.reshape(-1, sh[-1])
     if x2.shape[0] > MAX_ROWS:
         raise ValueError(f"mxfp4_linear: {x2.shape[0]} rows (at most {MAX_ROWS})")
-    if x.requires_grad and torch.is_grad_enabled():
-        if w.shape[0] > MAX_LD:
-            raise ValueError(f"mxfp4_linear: {w.shape[0]} columns with a gradient (at most {MAX_LD})")
-        y = _Linear.apply(x2, w, bias)
+    if x.requires_grad and torch.is_grad_enabled() and x.is_cuda:
+        (M, K), N = x2.shape, w.shape[0]
+        if N > MAX_LD:
+            raise ValueError(f"mxfp4_linear: {N} columns with a gradient (at most {MAX_LD})")
+        y = (_calls or _native_calls()).mx_linear_tracked(x2, w.data, N, bias, *_linear_form(M, N, K), *_grad_form(M, N, K))
     else:
         y = linear_rows(x2, w, bias)
     return y if len(sh) == 2 else y.view(*sh[:-1], w.shape[0])
@@ -382,14 +308,7 @@ def mxfp4_matmul(a: MXFP4, b: MXFP4, bias: Optional[torch.Tensor] = None, out_dt
     (M, K), dev = a.shape, a.data.device
     _check("mxfp4_matmul", K, dev, b, bias, out_dtype)
     N = b.shape[0]
-    if not use_seqmix(a.data):
+    if not a.data.is_cuda:
         y = _decode(a.codes, a.scales) @ _decode(b.codes, b.scales).t()
         return (y if bias is None else y + bias.float()).to(out_dtype)
-    y = torch.empty((M, N), dtype=out_dtype, device=dev)
-    if M and N:
-        if bias is not None:
-            bias = bias.contiguous()
-        tiles, m, n = _matmul_form(M, N, K)
-        _launch("sm_mx_matmul" if tiles else "sm_mx_rows_matmul", dev, DT[out_dtype], *_addresses(a), *_addresses(b),
-                0 if bias is None else bias.data_ptr(), y.data_ptr(), M, N, K, m, n)
-    return y
+    return (_calls or _native_calls()).mx_matmul(a.data, b.data, M, N, K, bias, out_dtype, *_matmul_form(M, N, K))
