@@ -141,7 +141,7 @@ hipError_t sm_mx_matmul(int dt, const void* xc, const void* xs, const void* code
     else if (dt == kF16) matmul_kernel<fp16, NI, MJ, 2><<<grid, 256, 0, st>>>(a);      \
     else matmul_kernel<float, NI, MJ, 2><<<grid, 256, 0, st>>>(a);                     \
     break;
-    GO(8, 4) GO(8, 8)
+    GO(8, 4) GO(8, 6) GO(8, 8)
 #undef GO
     default: return hipErrorInvalidValue;
   }

@@ -223,7 +223,7 @@ _MATMUL = ([(xr, 16 * rt, (0, xr, rt), (a + b * rt) / 2, f + g * rt)
             for xr, a, b, f, g, rts in ((16, 0.05, 0.0125, 2.9, 0.1, (1, 2, 4, 6, 8)), (32, 0.05, 0.015, 3.3, 0.1, (1, 2, 4, 6, 8)),
                                         (64, 0.087, 0.013, 2.8, 0.4, (1, 2, 3, 4, 6, 8)), (128, 0.0, 0.048, 0.0, 1.4, (4,)))
             for rt in rts]
-           + [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.36, 10.0), (8, 0.515, 15.7))])
+           + [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.36, 10.0), (6, 0.43, 12.0), (8, 0.515, 15.7))])
 
 
 @functools.lru_cache(4096)
