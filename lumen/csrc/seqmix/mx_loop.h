@@ -28,6 +28,16 @@ __device__ __forceinline__ void mfma(f32x4& c, uint4 a, uint4 b) {
 template <bool NAMED> __device__ __forceinline__ void settle() { if constexpr (NAMED) tile::settle(); }
 template <bool NAMED> __device__ __forceinline__ void hold(f32x4& c) { if constexpr (NAMED) tile::hold(c); }
 
+// LDS-DMA of 16 and 4 bytes per lane to lds + AT: three instructions, as they stand between products, where each costs its issue (with a
+// stage's addresses worked out for every piece of it 256 x 256 x 11008 of 4-bit operands took 87 us, so 55)
+template <int AT>
+__device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned lds) {
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(lds), "n"(AT) : "memory", "m0", "scc");
+}
+template <int AT>
+__device__ __forceinline__ void dma4(const void* base, unsigned off, unsigned lds) {
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" :: "v"(off), "s"(base), "s"(lds), "n"(AT) : "memory", "m0", "scc");
+}
 // LDS-DMA of 4 bytes per lane
 __device__ __forceinline__ void dma4(const void* base, unsigned off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
@@ -118,24 +128,40 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
   const int cx = (lane & 7) ^ ((4 * wid + (lane >> 4)) & 7);             // chunk of x that the lane brings
   const bool beyond = 8 * cx >= a.tail;
   const unsigned back = beyond ? 16 * cx : 0;
-  auto issue = [&](int t, int slot, int q0, int q1) __attribute__((always_inline)) {
-    const bool last = t == a.nk - 1;
-    const char* xs = a.x + (long long)t * 128;
-    const char* ws = GRAD ? a.w + (long long)t * 4096 : a.w + (t >> 1) * a.wp + (t & 1) * 32;
-    const char* ss = GRAD ? a.s + (long long)t * 256 : a.s + (t >> 1) * a.sp;
-    const unsigned d = __builtin_amdgcn_readfirstlane(lds0 + slot * SB + wid * 1024);
+  // the next stage to send for: its addresses and number; from the last on the same one again, into slots that nobody reads
+  const char *xs = a.x, *ws = a.w, *ss = a.s;
+  int sent = 0;
+  unsigned ox[PX], ow[PW], os = offs;
 #pragma unroll
-    for (int q = q0; q < q1; ++q) {
-      if (q < PX) tile::dma16(xs, offx[q] - (last ? back : 0u), d + q * 4096);
-      else if (q < PX + PW) {
-        const int u = q - PX;
-        const unsigned to = NW % 4 == 0 ? d + XB + u * 4096
-                                        : __builtin_amdgcn_readfirstlane(lds0 + slot * SB + XB + (wid + 4 * u) % NW * 1024);
-        tile::dma16(ws, GRAD && last ? lastw[u] : offw[u], to);
-      } else {
-        dma4(ss, GRAD && last ? lasts : offs, __builtin_amdgcn_readfirstlane(lds0 + slot * SB + XB + WB + wid * 256));
-      }
+  for (int q = 0; q < PX; ++q) ox[q] = offx[q];
+#pragma unroll
+  for (int q = 0; q < PW; ++q) ow[q] = offw[q];
+  auto begin = [&] __attribute__((always_inline)) {
+    if (sent != a.nk - 1) return;
+#pragma unroll
+    for (int q = 0; q < PX; ++q) ox[q] -= back;
+    if constexpr (GRAD) {
+#pragma unroll
+      for (int q = 0; q < PW; ++q) ow[q] = lastw[q];
+      os = lasts;
     }
+  };
+  auto piece = [&](auto num, unsigned d) __attribute__((always_inline)) {      // d: the wave's first KiB in the slot
+    constexpr int q = decltype(num)::value;
+    if constexpr (q < PX) dma16<q * 4096>(xs, ox[q], d);
+    else if constexpr (q < PX + PW) {
+      constexpr int u = q - PX;
+      if constexpr (NW % 4 == 0) dma16<XB + u * 4096>(ws, ow[u], d);
+      else dma16<XB>(ws, ow[u], d + ((wid + 4 * u) % NW - wid) * 1024);
+    } else {
+      dma4<XB + WB>(ss, os, d - wid * 768);
+    }
+  };
+  auto end = [&] __attribute__((always_inline)) {
+    const bool more = ++sent < a.nk, odd = sent & 1;
+    xs += more ? 128 : 0;
+    if constexpr (GRAD) ws += more ? 4096 : 0, ss += more ? 256 : 0;
+    else ws += more ? (odd ? 32 : a.wp - 32) : 0, ss += more && !odd ? a.sp : 0;
   };
   // what a last stage holds beyond the sum's end becomes zero; each wave mends the pieces that it sent for
   auto mend = [&](int slot) __attribute__((always_inline)) {
@@ -195,12 +221,12 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
       const uint2 v = columns<T, w>(raw[2 * u], raw[2 * u + 1], fs[0], fs[1]);
       fw[h][2 * w][u] = v.x, fw[h][2 * w + 1][u] = v.y;
     } else {
-      if constexpr (w == 0) fs[0] = mx_scale((sc[u] >> (16 * (t & 1) + 8 * h)) & 255u);
+      if constexpr (w == 0) fs[0] = mx_scale_of(sc[u], (9 + 8 * h + 16 * (t & 1)) & 31);
       fw[h][u][w] = pair<T, w>(raw[u], fs[0]);
     }
   };
-  // the products of half h, between them reads and making of the other half, of stage t2 in `slot`, and send(a, b): pieces a .. b - 1
-  auto half = [&](int h, int t2, int slot, auto&& send) __attribute__((always_inline)) {
+  // the products of half h, between them reads and making of the other half, of stage t2 in `slot`; SEND: and the DMA of a stage to d
+  auto half = [&](int h, int t2, int slot, auto send, unsigned d) __attribute__((always_inline)) {
     constexpr int U = NI * MJ, UR = (U * 3 + 7) / 8, UV = U < 48 ? U / 2 : U / 4;        // reads in products 0 .. UR - 1, making from UV on
     ready();
     each<0, U>([&](auto num) __attribute__((always_inline)) {
@@ -210,32 +236,38 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
       each<(r0 < READS ? r0 : READS), (r1 < READS ? r1 : READS)>([&](auto r) __attribute__((always_inline)) { read(1 - h, slot, r.value); });
       if constexpr (n >= UV)
         each<(n - UV) * UNITS / (U - UV), (n - UV + 1) * UNITS / (U - UV)>([&](auto r) __attribute__((always_inline)) { make(1 - h, t2, r); });
-      send(n * P / U, (n + 1) * P / U);
+      if constexpr (decltype(send)::value)
+        each<n * P / U, (n + 1) * P / U>([&](auto q) __attribute__((always_inline)) { piece(q, d); });
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  const auto none = [](int, int) __attribute__((always_inline)) {};
   const int nk = a.nk;
+  const unsigned d0 = __builtin_amdgcn_readfirstlane(lds0 + wid * 1024);
 #pragma unroll
-  for (int u = 0; u < NST; ++u)
-    if (u < nk) issue(u, u, 0, P);
+  for (int u = 0; u < NST; ++u) {
+    begin();
+    each<0, P>([&](auto q) __attribute__((always_inline)) { piece(q, d0 + u * SB); });
+    end();
+  }
   // stage 0 has arrived
-  tile::wait_stages<NST - 1, P>(nk - 1);
+  tile::wait_vm<(NST - 1) * P>();
   if (nk == 1) mend(0);
   tile::done_reading();
 #pragma unroll
   for (int r = 0; r < READS; ++r) read(0, 0, r);
   each<0, UNITS>([&](auto r) __attribute__((always_inline)) { make(0, 0, r); });
   for (int t = 0, s0 = 0, s1 = 1;;) {                    // slots of stages t and t + 1
-    half(0, t, s0, none);
-    tile::wait_stages<NST - 2, P>(nk - 2 - t);           // stage t + 1 has arrived
+    half(0, t, s0, Int<0>{}, 0u);
+    tile::wait_vm<(NST - 2) * P>();                      // stage t + 1 has arrived
     if (t + 2 == nk) mend(s1);
     tile::done_reading();
-    const bool more = t + NST < nk;
-    half(1, t + 1, s1, [&](int b, int e) __attribute__((always_inline)) { if (more) issue(t + NST, s0, b, e); });
+    begin();
+    half(1, t + 1, s1, Int<1>{}, __builtin_amdgcn_readfirstlane(d0 + s0 * SB));
+    end();
     s0 = s1, s1 = s1 == NST - 1 ? 0 : s1 + 1;            // (the last step reads a slot that holds an earlier stage, or none: unused)
     if (++t == nk) break;
   }
+  tile::wait_vm<0>();                                    // (nothing of this workgroup is under way when its LDS is another's)
   settle<NAMED>();
 }
 
@@ -249,7 +281,7 @@ struct Shape4 {
   static constexpr int XB = BM * 64, WB = BN * 64, SB = XB + WB + 2048;
   static constexpr int NX = BM / 16, NW = BN / 16, PX = (NX + 3) / 4, PW = (NW + 3) / 4, PIECES = PX + PW + 2;
   static constexpr int FIT = kLds / SB, NST = FIT < 6 ? FIT : 6, LDS = NST * SB;
-  static_assert(BM <= 256 && BN <= 256 && NST >= 3 && (NST - 1) * PIECES < 64, "tile");
+  static_assert(BM <= 256 && BM % 64 == 0 && BN <= 256 && NST >= 3 && (NST - 1) * PIECES < 64, "tile");
 };
 
 struct Walk4 {
@@ -274,22 +306,26 @@ __device__ __forceinline__ void products4(char* lds, const Walk4& a, const unsig
                                           const unsigned (&offw)[Shape4<NI, MJ, WN>::PW], unsigned offs, f32x4 (&acc)[NI][MJ]) {
   using S = Shape4<NI, MJ, WN>;
   constexpr bool NAMED = kNamed<NI, MJ>;
-  constexpr int PX = S::PX, PW = S::PW, NX = S::NX, NW = S::NW, P = S::PIECES, NST = S::NST, SB = S::SB, XB = S::XB, WB = S::WB;
+  constexpr int PX = S::PX, PW = S::PW, NW = S::NW, P = S::PIECES, NST = S::NST, SB = S::SB, XB = S::XB, WB = S::WB;
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wid / WN, wn = wid % WN;
   const unsigned lds0 = lds_addr(lds);
-  auto issue = [&](int u, int slot, int q0, int q1) __attribute__((always_inline)) {
-    const unsigned d = lds0 + slot * SB;
-    const int t = min(u, a.nk - 1);
-#pragma unroll
-    for (int q = q0; q < q1; ++q) {
-      if (q < PX) tile::dma16(a.x + t * a.xp, offx[q], __builtin_amdgcn_readfirstlane(d + (wid + 4 * q) % NX * 1024));
-      else if (q < PX + PW)
-        tile::dma16(a.w + t * a.wp, offw[q - PX], __builtin_amdgcn_readfirstlane(d + XB + (wid + 4 * (q - PX)) % NW * 1024));
-      else if (q == PX + PW) dma4(a.xs + t * a.xsp, offxs, __builtin_amdgcn_readfirstlane(d + XB + WB + wid * 256));
-      else dma4(a.s + t * a.sp, offs, __builtin_amdgcn_readfirstlane(d + XB + WB + 1024 + wid * 256));
-    }
+  const char *px = a.x, *pxs = a.xs, *pw = a.w, *ps = a.s;               // the next panel to send for, from the last on that one again
+  int sent = 0;
+  auto piece = [&](auto num, unsigned d) __attribute__((always_inline)) {      // d: the wave's first KiB in the slot
+    constexpr int q = decltype(num)::value;
+    if constexpr (q < PX) dma16<q * 4096>(px, offx[q], d);
+    else if constexpr (q < PX + PW) {
+      constexpr int u = q - PX;
+      if constexpr (NW % 4 == 0) dma16<XB + u * 4096>(pw, offw[u], d);
+      else dma16<XB>(pw, offw[u], d + ((wid + 4 * u) % NW - wid) * 1024);
+    } else if constexpr (q == PX + PW) dma4<XB + WB>(pxs, offxs, d - wid * 768);
+    else dma4<XB + WB + 1024>(ps, offs, d - wid * 768);
+  };
+  auto end = [&] __attribute__((always_inline)) {
+    const bool more = ++sent < a.nk;
+    px += more ? a.xp : 0, pxs += more ? a.xsp : 0, pw += more ? a.wp : 0, ps += more ? a.sp : 0;
   };
 #pragma unroll
   for (int i = 0; i < NI; ++i)
@@ -311,7 +347,7 @@ __device__ __forceinline__ void products4(char* lds, const Walk4& a, const unsig
     if (n < NI) asm volatile("v_lshrrev_b32 %0, %1, %0" : "+v"(sw[h][n]) : "v"(8 * lg));
     else asm volatile("v_lshrrev_b32 %0, %1, %0" : "+v"(sx[h][n - NI]) : "v"(8 * lg));
   };
-  auto step = [&](int h, int slot, auto&& send) __attribute__((always_inline)) {
+  auto step = [&](int h, int slot, unsigned d) __attribute__((always_inline)) {
     constexpr int U = NI * MJ, UR = (U * 5 + 7) / 8, UV = U / 2;
     ready();
     each<0, U>([&](auto num) __attribute__((always_inline)) {
@@ -321,16 +357,19 @@ __device__ __forceinline__ void products4(char* lds, const Walk4& a, const unsig
       each<(r0 < READS ? r0 : READS), (r1 < READS ? r1 : READS)>([&](auto r) __attribute__((always_inline)) { read(1 - h, slot, r.value); });
       if constexpr (n >= UV)
         each<(n - UV) * UNITS / (U - UV), (n - UV + 1) * UNITS / (U - UV)>([&](auto r) __attribute__((always_inline)) { make(1 - h, r.value); });
-      send(n * P / U, (n + 1) * P / U);
+      each<n * P / U, (n + 1) * P / U>([&](auto q) __attribute__((always_inline)) { piece(q, d); });
       __builtin_amdgcn_sched_barrier(0);
     });
   };
   // two panels a way round, the second one zeros where there is none: the loop has one way out (accumulators, above)
   const int nk = (a.nk + 1) & ~1;
+  const unsigned d0 = __builtin_amdgcn_readfirstlane(lds0 + wid * 1024);
 #pragma unroll
-  for (int u = 0; u < NST; ++u)
-    if (u < nk) issue(u, u, 0, P);
-  tile::wait_stages<NST - 1, P>(nk - 1);
+  for (int u = 0; u < NST; ++u) {
+    each<0, P>([&](auto q) __attribute__((always_inline)) { piece(q, d0 + u * SB); });
+    end();
+  }
+  tile::wait_vm<(NST - 1) * P>();
   tile::done_reading();
 #pragma unroll
   for (int r = 0; r < READS; ++r) read(0, 0, r);
@@ -338,18 +377,19 @@ __device__ __forceinline__ void products4(char* lds, const Walk4& a, const unsig
   for (int r = 0; r < UNITS; ++r) make(0, r);
   int t = 0, s0 = 0, s1 = 1;
   auto next = [&](int h) __attribute__((always_inline)) {
-    tile::wait_stages<NST - 2, P>(nk - 2 - t);           // panel t + 1 has arrived
+    tile::wait_vm<(NST - 2) * P>();                      // panel t + 1 has arrived
     if (t + 1 == a.nk) {                                 // (each wave clears what it sent for)
 #pragma unroll
-      for (int q = 0; q < PX; ++q) *reinterpret_cast<uint4*>(lds + s1 * SB + (wid + 4 * q) % NX * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
+      for (int q = 0; q < PX; ++q) *reinterpret_cast<uint4*>(lds + s1 * SB + (wid + 4 * q) * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
     }
     tile::done_reading();
-    const bool more = t + NST < nk;
-    step(h, s1, [&](int b, int e) __attribute__((always_inline)) { if (more) issue(t + NST, s0, b, e); });
+    step(h, s1, __builtin_amdgcn_readfirstlane(d0 + s0 * SB));
+    end();
     s0 = s1, s1 = s1 == NST - 1 ? 0 : s1 + 1, ++t;
   };
   do next(0), next(1);
   while (t < nk);
+  tile::wait_vm<0>();                                    // (nothing of this workgroup is under way when its LDS is another's)
   settle<NAMED>();
 }
 
