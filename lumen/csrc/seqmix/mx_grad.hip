@@ -33,9 +33,10 @@ __global__ void __launch_bounds__(256, 1) grad_kernel(const TileArgs a) {
   }
   const unsigned as = (unsigned)min(wid % WN, panels - 1 - panel) * (unsigned)sp;
   const mx::Walk walk{(const char*)a.x + (long long)m0 * a.ldx * 2, (const char*)a.codes + panel * wp, (const char*)a.scales + panel * sp,
-                      wp, sp, nk, a.Nx - 64 * (nk - 1), left};
+                      wp, sp, nk, a.Nx - 64 * (nk - 1), left, 0};
+  const unsigned offs[1] = {as + 4 * lane}, lasts[1] = {as + 4 * min(lane, left - 1)};
   f32x4 acc[8][MJ];
-  mx::products<T, 8, MJ, WN, true>(lds, walk, offx, offw, as + 4 * lane, lastw, as + 4 * min(lane, left - 1), acc);
+  mx::products<T, 8, MJ, WN, true>(lds, walk, offx, offw, offs, lastw, lasts, acc);
 #pragma unroll
   for (int j = 0; j < MJ; ++j) {
     const int m = m0 + 16 * MJ * (wid / WN) + 16 * j + lr;
@@ -50,121 +51,50 @@ __global__ void __launch_bounds__(256, 1) grad_kernel(const TileArgs a) {
   }
 }
 
-// Few results: a workgroup takes XR rows of dy and one panel of columns, its NW waves split the sum over w's rows (seqmix/mx_rows.hip has
-// the ring); a wave's stage is 64 of them.
-template <int XR, int NW, int D>
-struct Ring {
-  static constexpr int MT = XR / 16, XB = XR * 128, XP = XB / 1024, SB = XB + 4096 + 256, G = XP + 5, PART = 8 * MT * 1024;
-  static constexpr int LDS = NW * D * SB > NW * PART ? NW * D * SB : NW * PART;
-  static_assert(XR % 16 == 0 && LDS <= mx::kLds && D >= 2 && G * (D - 1) < 64, "ring");
-};
-
-template <typename T, int XR, int NW, int D>
+// Few results: a workgroup takes 16 MT rows of dy and one panel of columns, its NW waves split the sum over w's rows, each in a ring of its own.
+template <typename T, int MT, int NW>
 __global__ void __launch_bounds__(64 * NW, 1) rows_grad_kernel(const TileArgs a) {
-  using S = Ring<XR, NW, D>;
-  constexpr int MT = S::MT, XP = S::XP, XB = S::XB, G = S::G;
-  __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+  using S = mx::Shape<8, MT, -NW, true>;
+  constexpr int XR = 16 * MT, PART = 8 * MT * 1024;
+  __shared__ __attribute__((aligned(16))) char lds[NW * (S::LDS > PART ? S::LDS : PART)];
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = tile::unit_of(blockIdx.x, gridDim.x);
   const int tm = tile % a.tiles_m, panel = tile / a.tiles_m;
   const int m0 = tm * XR;
-  char* ring = lds + wid * D * S::SB;
-  const unsigned ring0 = __builtin_amdgcn_readfirstlane(mx::lds_addr(ring));
   const int steps = (a.N + 63) / 64, t0 = steps * wid / NW, nk = steps * (wid + 1) / NW - t0;
-  const int tail = a.Nx - 64 * (steps - 1), left = a.N - 64 * (steps - 1);
-  const char* xb = (const char*)a.x + (long long)m0 * a.ldx * 2;
-  const char* wb = (const char*)a.codes + (long long)panel * a.N * 64;
-  const char* sb = (const char*)a.scales + (long long)panel * a.N * 4;
-  unsigned offx[XP], offw[4], lastw[4];
-#pragma unroll
-  for (int q = 0; q < XP; ++q) {
-    const int r = 8 * q + (lane >> 3);
-    offx[q] = (unsigned)min(r, a.M - m0 - 1) * (unsigned)(2 * a.ldx) + 16 * ((lane & 7) ^ tile::swz(r));
-  }
-  auto row = [&](int q) {                                // of w, that the lane brings with piece q: rows 8 apart lie side by side
-    const int pos = 16 * (q & 1) + (lane >> 2);
-    return 32 * (q >> 1) + ((pos & 3) << 3 | pos >> 2);
-  };
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    offw[q] = 64 * row(q) + 16 * (lane & 3);
-    lastw[q] = 64 * min(row(q), left - 1) + 16 * (lane & 3);
-  }
-  auto issue = [&](int i) __attribute__((always_inline)) {
-    const int t = t0 + i;
-    const bool last = t == steps - 1;
-    const unsigned d = ring0 + i % D * S::SB;
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      tile::dma16(wb + (long long)t * 4096, last ? lastw[q] : offw[q], __builtin_amdgcn_readfirstlane(d + XB + q * 1024));
-    mx::dma4(sb + (long long)t * 256, 4 * (last ? min(lane, left - 1) : lane), __builtin_amdgcn_readfirstlane(d + XB + 4096));
-#pragma unroll
-    for (int q = 0; q < XP; ++q) {
-      const int c = (lane & 7) ^ tile::swz(8 * q + (lane >> 3));
-      tile::dma16(xb + (long long)t * 128, offx[q] - (last && 8 * c >= tail ? 16 * c : 0), __builtin_amdgcn_readfirstlane(d + q * 1024));
-    }
-  };
   f32x4 acc[8][MT];
+  if (nk > 0) {
+    const bool last = t0 + nk == steps;
+    const int tail = last ? a.Nx - 64 * (steps - 1) : 64, left = last ? a.N - 64 * (steps - 1) : 64;
+    unsigned offx[S::PX], offw[4], lastw[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < D - 1; ++i)
-    if (i < nk) issue(i);
-  for (int i = 0; i < nk; ++i) {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the fragments of stage i - 1 have been read: its slot may be filled again)
-    if (i + D - 1 < nk) issue(i + D - 1);
-    tile::wait_stages<D - 1, G>(nk - 1 - i);             // stage i has arrived
-    asm volatile("" ::: "memory");
-    char* img = ring + i % D * S::SB;
-    if (t0 + i == steps - 1 && left < 64) {              // what lies beyond w's rows: zeros
-#pragma unroll
-      for (int q = 0; q < XP; ++q)
-        if (8 * ((lane & 7) ^ tile::swz(8 * q + (lane >> 3))) >= tail) *reinterpret_cast<uint4*>(img + q * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (row(q) >= left) *reinterpret_cast<uint4*>(img + XB + q * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
-      if (lane >= left) *reinterpret_cast<unsigned*>(img + XB + 4096 + lane * 4) = 0;
+    for (int q = 0; q < S::PX; ++q) {
+      const int r = 8 * q + (lane >> 3);
+      offx[q] = (unsigned)min(r, a.M - m0 - 1) * (unsigned)(2 * a.ldx) + 16 * ((lane & 7) ^ tile::swz(r));
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      unsigned raw[8], fw[8][4];
-      float sc[8];
-      uint4 fx[MT];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        raw[r] = *reinterpret_cast<const unsigned*>(img + XB + h * 2048 + (4 * r + lg) * 64 + lr * 4);
-        sc[r] = mx_scale(*reinterpret_cast<const unsigned char*>(img + XB + 4096 + (32 * h + 8 * lg + r) * 4 + (lr >> 2)));
-      }
-#pragma unroll
-      for (int j = 0; j < MT; ++j)
-        fx[j] = *reinterpret_cast<const uint4*>(img + (16 * j + lr) * 128 + (((4 * h + lg) ^ tile::swz(lr)) << 4));
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint2 v0 = mx::columns<T, 0>(raw[2 * u], raw[2 * u + 1], sc[2 * u], sc[2 * u + 1]);
-        const uint2 v1 = mx::columns<T, 1>(raw[2 * u], raw[2 * u + 1], sc[2 * u], sc[2 * u + 1]);
-        const uint2 v2 = mx::columns<T, 2>(raw[2 * u], raw[2 * u + 1], sc[2 * u], sc[2 * u + 1]);
-        const uint2 v3 = mx::columns<T, 3>(raw[2 * u], raw[2 * u + 1], sc[2 * u], sc[2 * u + 1]);
-        fw[0][u] = v0.x, fw[1][u] = v0.y, fw[2][u] = v1.x, fw[3][u] = v1.y;
-        fw[4][u] = v2.x, fw[5][u] = v2.y, fw[6][u] = v3.x, fw[7][u] = v3.y;
-      }
-      mx::ready();
-#pragma unroll
-      for (int i8 = 0; i8 < 8; ++i8) {
-        const uint4 w = make_uint4(fw[i8][0], fw[i8][1], fw[i8][2], fw[i8][3]);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i8][j] = Mfma<T>::run(w, fx[j], acc[i8][j]);
-      }
+    for (int q = 0; q < 4; ++q) {
+      const int pos = 16 * (q & 1) + (lane >> 2), n = 32 * (q >> 1) + ((pos & 3) << 3 | pos >> 2);
+      offw[q] = 64 * n + 16 * (lane & 3);
+      lastw[q] = 64 * min(n, left - 1) + 16 * (lane & 3);
     }
+    const unsigned offs[1] = {4u * lane}, lasts[1] = {4u * min(lane, left - 1)};
+    const mx::Walk walk{(const char*)a.x + (long long)m0 * a.ldx * 2 + (long long)t0 * 128, (const char*)a.codes + (long long)panel * a.N * 64 + (long long)t0 * 4096,
+                        (const char*)a.scales + (long long)panel * a.N * 4 + (long long)t0 * 256, 0, 0, nk, tail, left, 0};
+    mx::products<T, 8, MT, -NW, true>(lds + wid * S::LDS, walk, offx, offw, offs, lastw, lasts, acc);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   // the waves' sums, over the rings
   tile::done_reading();
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(lds + wid * S::PART + (i * MT + j) * 1024 + lane * 16) = acc[i][j];
+    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(lds + wid * PART + (i * MT + j) * 1024 + lane * 16) = acc[i][j];
   __syncthreads();
   for (int q = wid; q < 4 * MT; q += NW) {               // row 4 lg + e of fragment i: column 8 (4 lg + e) + i
     const int j = q >> 2, e = q & 3, m = m0 + 16 * j + lr, k = 128 * panel + 32 * lg + 8 * e;
@@ -173,7 +103,7 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_grad_kernel(const TileArgs a)
     for (int i = 0; i < 8; ++i) {
       r[i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) r[i] += *reinterpret_cast<const float*>(lds + w * S::PART + (i * MT + j) * 1024 + lane * 16 + 4 * e);
+      for (int w = 0; w < NW; ++w) r[i] += *reinterpret_cast<const float*>(lds + w * PART + (i * MT + j) * 1024 + lane * 16 + 4 * e);
     }
     if (m < a.M && k < a.K) store8((T*)a.y + (long long)m * a.K + k, r);
   }
@@ -217,12 +147,12 @@ hipError_t sm_mx_rows_grad(int dt, const void* dy, long long ldy, const void* co
   int grid;
   if (!mx::plan(a, K, xr, 128, grid)) return hipErrorInvalidValue;
   switch (xr) {
-#define GO(XR, NW, D)                                                                          \
+#define GO(XR, NW)                                                                             \
   case XR:                                                                                     \
-    if (dt == kBF16) rows_grad_kernel<bf16, XR, NW, D><<<grid, 64 * NW, 0, st>>>(a);           \
-    else rows_grad_kernel<fp16, XR, NW, D><<<grid, 64 * NW, 0, st>>>(a);                       \
+    if (dt == kBF16) rows_grad_kernel<bf16, XR / 16, NW><<<grid, 64 * NW, 0, st>>>(a);         \
+    else rows_grad_kernel<fp16, XR / 16, NW><<<grid, 64 * NW, 0, st>>>(a);                     \
     break;
-    GO(16, 8, 3) GO(32, 4, 4) GO(64, 4, 3)
+    GO(16, 8) GO(32, 4) GO(64, 4)
 #undef GO
     default: return hipErrorInvalidValue;
   }

@@ -16,7 +16,7 @@ __global__ void __launch_bounds__(256, 1) linear_kernel(const TileArgs a) {
   tile::tile_at(tile::unit_of(blockIdx.x, gridDim.x), a.tiles_m, a.tiles_n, a.group, tm, tn);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   auto column = [&](int r) { return min(n0 + r / (16 * NI) * (16 * NI) + tile::colperm<NI>(r % (16 * NI)), a.N - 1); };
-  unsigned offx[S::PX], offw[S::PW], offs;
+  unsigned offx[S::PX], offw[S::PW], offs[1];
 #pragma unroll
   for (int q = 0; q < S::PX; ++q) {                      // (rows past the edge read the last row: never stored)
     const int r = 8 * (wid + 4 * q) + (lane >> 3);
@@ -25,10 +25,10 @@ __global__ void __launch_bounds__(256, 1) linear_kernel(const TileArgs a) {
 #pragma unroll
   for (int q = 0; q < S::PW; ++q)
     offw[q] = (unsigned)column((wid + 4 * q) % S::NW * 32 + (lane >> 1)) * 64u + 16 * ((lane ^ lane >> 4) & 1);
-  offs = (unsigned)column(min(64 * wid + lane, S::BN - 1)) * 4u;
+  offs[0] = (unsigned)column(min(64 * wid + lane, S::BN - 1)) * 4u;
   const int nk = (a.K + 63) / 64;
   const mx::Walk walk{(const char*)a.x + (long long)m0 * a.ldx * 2, (const char*)a.codes, (const char*)a.scales, (long long)a.N * 64,
-                      (long long)a.N * 4, nk, a.K - 64 * (nk - 1), 64};
+                      (long long)a.N * 4, nk, a.K - 64 * (nk - 1), 64, 0};
   f32x4 acc[NI][MJ];
   mx::products<T, NI, MJ, WN, false>(lds, walk, offx, offw, offs, offw, offs, acc);
   mx::put_all<T, NI, MJ>(a, acc, m0 + 16 * MJ * (wid / WN), n0 + 16 * NI * (wid % WN));

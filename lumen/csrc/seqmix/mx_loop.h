@@ -94,71 +94,80 @@ __device__ __forceinline__ uint2 columns(unsigned c0, unsigned c1, float s0, flo
 //  * GRAD false: y = x w^T.  A fragment of w is 16 of its rows by 32 k, one block a row: a lane reads four bytes, its 8 codes.
 //  * GRAD true: dx = dy w, the sum runs over w's rows.  A lane takes 8 rows' codes of the 8 columns it stands for; two rows' pairs
 //    are regrouped by column (v_perm), which gives 8 fragments, of columns 8 a + j for j = 0 .. 7 (a: row of the fragment).
+// WN = -4 or -8: one wave's 16 MJ x 16 NI, in a ring of its own among the 4 or 8 waves of a workgroup that split the sum: no barriers.
 template <int NI, int MJ, int WN, bool GRAD>
 struct Shape {
-  static constexpr int WM = 4 / WN, BM = 16 * MJ * WM, BN = 16 * NI * WN;
-  static constexpr int XB = BM * 128, WB = BN * 32, SB = XB + WB + 1024;      // a stage: x, codes, scales
-  static constexpr int PX = BM / 32, NW = BN / 32, PW = (NW + 3) / 4, PIECES = PX + PW + 1;
-  static constexpr int FIT = kLds / SB, NST = FIT < 6 ? FIT : 6, LDS = NST * SB;
-  static_assert(BM % 32 == 0 && BN % 32 == 0 && BN <= 256 && NST >= 3 && (NST - 1) * PIECES < 64, "tile");
+  static constexpr bool OWN = WN < 0;
+  static constexpr int WM = OWN ? 1 : 4 / WN, BM = 16 * MJ * WM, BN = 16 * NI * (OWN ? 1 : WN);
+  static constexpr int NW = OWN ? (GRAD ? 4 : (NI + 1) / 2) : BN / 32;        // KiB of codes in a stage
+  // a wave's pieces of x, codes and scales, and what lies between two of them
+  static constexpr int PX = OWN ? BM / 8 : BM / 32, PW = OWN ? NW : (NW + 3) / 4, PS = OWN && !GRAD ? (NI + 3) / 4 : 1;
+  static constexpr int STEP = OWN ? 1024 : 4096, PIECES = PX + PW + PS;
+  static constexpr int XB = BM * 128, WB = NW * 1024, SB = XB + WB + (OWN ? 256 * PS : 1024);      // a stage: x, codes, scales
+  static constexpr int FIT = kLds / ((OWN ? -WN : 1) * SB), NST = FIT < 6 ? FIT : 6, LDS = NST * SB;
+  static_assert((OWN || (BM % 32 == 0 && BN % 32 == 0 && BN <= 256)) && NST >= 3 && (NST - 1) * PIECES < 64, "tile");
   static_assert(!GRAD || NI == 8, "a panel a wave");
 };
 
 struct Walk {
   const char* x;              // first row of the tile, 2-byte elements, 128 bytes a stage
-  const char *w, *s;          // codes and scales: of panel 0 and row 0 (GRAD: of the tile's first panel)
+  const char *w, *s;          // codes and scales: of the first stage and row 0 (GRAD: of the tile's first panel)
   long long wp, sp;           // bytes from panel to panel
   int nk, tail, tailw;        // stages; values of x in the last one (a multiple of 8); GRAD: rows of w in it
+  int odd;                    // 1: the first stage is the second half of a panel
 };
 
-// acc[i][j] += products of fragments i of w and j of x.  offx[q], offw[q], offs: the lane's byte offsets of its pieces; lastw, lasts: of
+// acc[i][j] += products of fragments i of w and j of x.  offx[q], offw[q], offs[q]: the lane's byte offsets of its pieces; lastw, lasts: of
 // those of the last stage (GRAD), whose rows from `tail` on are not w's own.
 template <typename T, int NI, int MJ, int WN, bool GRAD>
 __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigned (&offx)[Shape<NI, MJ, WN, GRAD>::PX],
-                                         const unsigned (&offw)[Shape<NI, MJ, WN, GRAD>::PW], unsigned offs,
-                                         const unsigned (&lastw)[Shape<NI, MJ, WN, GRAD>::PW], unsigned lasts,
-                                         f32x4 (&acc)[NI][MJ]) {
+                                         const unsigned (&offw)[Shape<NI, MJ, WN, GRAD>::PW],
+                                         const unsigned (&offs)[Shape<NI, MJ, WN, GRAD>::PS],
+                                         const unsigned (&lastw)[Shape<NI, MJ, WN, GRAD>::PW],
+                                         const unsigned (&lasts)[Shape<NI, MJ, WN, GRAD>::PS], f32x4 (&acc)[NI][MJ]) {
   using S = Shape<NI, MJ, WN, GRAD>;
-  constexpr bool NAMED = kNamed<NI, MJ>;
-  constexpr int PX = S::PX, PW = S::PW, NW = S::NW, P = S::PIECES, NST = S::NST, SB = S::SB, XB = S::XB, WB = S::WB;
+  constexpr bool NAMED = kNamed<NI, MJ>, OWN = S::OWN;
+  constexpr int PX = S::PX, PW = S::PW, PS = S::PS, NW = S::NW, P = S::PIECES, NST = S::NST, SB = S::SB, XB = S::XB, WB = S::WB;
+  constexpr int STEP = S::STEP, P1 = (P + 1) / 2;
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
-  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wid / WN, wn = wid % WN;
+  const int wid = OWN ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = OWN ? 0 : wid / (OWN ? 1 : WN), wn = OWN ? 0 : wid % (OWN ? 1 : WN);
   const unsigned lds0 = lds_addr(lds);
-  const int cx = (lane & 7) ^ ((4 * wid + (lane >> 4)) & 7);             // chunk of x that the lane brings
-  const bool beyond = 8 * cx >= a.tail;
-  const unsigned back = beyond ? 16 * cx : 0;
+  auto chunk = [&](int q) { return (lane & 7) ^ ((4 * (OWN ? q : wid) + (lane >> 4)) & 7); };            // of x, that the lane brings
   // the next stage to send for: its addresses and number; from the last on the same one again, into slots that nobody reads
   const char *xs = a.x, *ws = a.w, *ss = a.s;
   int sent = 0;
-  unsigned ox[PX], ow[PW], os = offs;
+  unsigned ox[PX], ow[PW], os[PS];
 #pragma unroll
   for (int q = 0; q < PX; ++q) ox[q] = offx[q];
 #pragma unroll
   for (int q = 0; q < PW; ++q) ow[q] = offw[q];
+#pragma unroll
+  for (int q = 0; q < PS; ++q) os[q] = offs[q];
   auto begin = [&] __attribute__((always_inline)) {
     if (sent != a.nk - 1) return;
 #pragma unroll
-    for (int q = 0; q < PX; ++q) ox[q] -= back;
+    for (int q = 0; q < PX; ++q) ox[q] -= 8 * chunk(q) >= a.tail ? 16 * chunk(q) : 0;
     if constexpr (GRAD) {
 #pragma unroll
       for (int q = 0; q < PW; ++q) ow[q] = lastw[q];
-      os = lasts;
+#pragma unroll
+      for (int q = 0; q < PS; ++q) os[q] = lasts[q];
     }
   };
   auto piece = [&](auto num, unsigned d) __attribute__((always_inline)) {      // d: the wave's first KiB in the slot
     constexpr int q = decltype(num)::value;
-    if constexpr (q < PX) dma16<q * 4096>(xs, ox[q], d);
+    if constexpr (q < PX) dma16<q * STEP>(xs, ox[q], d);
     else if constexpr (q < PX + PW) {
       constexpr int u = q - PX;
-      if constexpr (NW % 4 == 0) dma16<XB + u * 4096>(ws, ow[u], d);
+      if constexpr (OWN || NW % 4 == 0) dma16<XB + u * STEP>(ws, ow[u], d);
       else dma16<XB>(ws, ow[u], d + ((wid + 4 * u) % NW - wid) * 1024);
     } else {
-      dma4<XB + WB>(ss, os, d - wid * 768);
+      dma4<XB + WB + (q - PX - PW) * 256>(ss, os[q - PX - PW], d - wid * 768);
     }
   };
   auto end = [&] __attribute__((always_inline)) {
-    const bool more = ++sent < a.nk, odd = sent & 1;
+    const bool more = ++sent < a.nk, odd = (sent + a.odd) & 1;
     xs += more ? 128 : 0;
     if constexpr (GRAD) ws += more ? 4096 : 0, ss += more ? 256 : 0;
     else ws += more ? (odd ? 32 : a.wp - 32) : 0, ss += more && !odd ? a.sp : 0;
@@ -167,19 +176,23 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
   auto mend = [&](int slot) __attribute__((always_inline)) {
     if (a.tail == 64 && (!GRAD || a.tailw == 64)) return;
     char* d = lds + slot * SB;
-    if (beyond) {
 #pragma unroll
-      for (int q = 0; q < PX; ++q) *reinterpret_cast<uint4*>(d + wid * 1024 + q * 4096 + lane * 16) = make_uint4(0, 0, 0, 0);
-    }
+    for (int q = 0; q < PX; ++q)
+      if (8 * chunk(q) >= a.tail) *reinterpret_cast<uint4*>(d + wid * 1024 + q * STEP + lane * 16) = make_uint4(0, 0, 0, 0);
     if constexpr (GRAD) {
 #pragma unroll
       for (int u = 0; u < PW; ++u) {
-        const int pc = (wid + 4 * u) % NW, pos = 16 * (pc & 1) + (lane >> 2);
+        const int pc = OWN ? u : (wid + 4 * u) % NW, pos = 16 * (pc & 1) + (lane >> 2);
         if (32 * ((pc >> 1) & 1) + ((pos & 3) << 3 | pos >> 2) >= a.tailw)
           *reinterpret_cast<uint4*>(d + XB + pc * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
       }
       if (lane >= a.tailw) *reinterpret_cast<unsigned*>(d + XB + WB + wid * 256 + lane * 4) = 0;
     }
+  };
+  // the wave's reads have arrived, and (not OWN) every wave's
+  auto done = [&] __attribute__((always_inline)) {
+    if constexpr (OWN) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    else tile::done_reading();
   };
 #pragma unroll
   for (int i = 0; i < NI; ++i)
@@ -221,13 +234,14 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
       const uint2 v = columns<T, w>(raw[2 * u], raw[2 * u + 1], fs[0], fs[1]);
       fw[h][2 * w][u] = v.x, fw[h][2 * w + 1][u] = v.y;
     } else {
-      if constexpr (w == 0) fs[0] = mx_scale_of(sc[u], (9 + 8 * h + 16 * (t & 1)) & 31);
+      if constexpr (w == 0) fs[0] = mx_scale_of(sc[u], (9 + 8 * h + 16 * ((t + a.odd) & 1)) & 31);
       fw[h][u][w] = pair<T, w>(raw[u], fs[0]);
     }
   };
-  // the products of half h, between them reads and making of the other half, of stage t2 in `slot`; SEND: and the DMA of a stage to d
-  auto half = [&](int h, int t2, int slot, auto send, unsigned d) __attribute__((always_inline)) {
+  // the products of half h, between them reads and making of the other half, of stage t2 in `slot`, and pieces A .. B - 1 of a stage to d
+  auto half = [&](int h, int t2, int slot, auto from, auto to, unsigned d) __attribute__((always_inline)) {
     constexpr int U = NI * MJ, UR = (U * 3 + 7) / 8, UV = U < 48 ? U / 2 : U / 4;        // reads in products 0 .. UR - 1, making from UV on
+    constexpr int A = decltype(from)::value, N = decltype(to)::value - A;
     ready();
     each<0, U>([&](auto num) __attribute__((always_inline)) {
       constexpr int n = decltype(num)::value, i = n % NI, j = n / NI;
@@ -236,34 +250,36 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
       each<(r0 < READS ? r0 : READS), (r1 < READS ? r1 : READS)>([&](auto r) __attribute__((always_inline)) { read(1 - h, slot, r.value); });
       if constexpr (n >= UV)
         each<(n - UV) * UNITS / (U - UV), (n - UV + 1) * UNITS / (U - UV)>([&](auto r) __attribute__((always_inline)) { make(1 - h, t2, r); });
-      if constexpr (decltype(send)::value)
-        each<n * P / U, (n + 1) * P / U>([&](auto q) __attribute__((always_inline)) { piece(q, d); });
+      each<A + n * N / U, A + (n + 1) * N / U>([&](auto q) __attribute__((always_inline)) { piece(q, d); });
       __builtin_amdgcn_sched_barrier(0);
     });
   };
   const int nk = a.nk;
   const unsigned d0 = __builtin_amdgcn_readfirstlane(lds0 + wid * 1024);
-#pragma unroll
-  for (int u = 0; u < NST; ++u) {
+  each<0, NST>([&](auto slot) __attribute__((always_inline)) {
+    constexpr int u = decltype(slot)::value;
     begin();
-    each<0, P>([&](auto q) __attribute__((always_inline)) { piece(q, d0 + u * SB); });
-    end();
-  }
+    each<0, (u < NST - 1 ? P : P1)>([&](auto q) __attribute__((always_inline)) { piece(q, d0 + u * SB); });
+    if constexpr (u < NST - 1) end();
+  });
   // stage 0 has arrived
-  tile::wait_vm<(NST - 1) * P>();
+  tile::wait_vm<(NST - 2) * P + P1>();
   if (nk == 1) mend(0);
-  tile::done_reading();
+  done();
 #pragma unroll
   for (int r = 0; r < READS; ++r) read(0, 0, r);
   each<0, UNITS>([&](auto r) __attribute__((always_inline)) { make(0, 0, r); });
-  for (int t = 0, s0 = 0, s1 = 1;;) {                    // slots of stages t and t + 1
-    half(0, t, s0, Int<0>{}, 0u);
+  // slots of stages t and t + 1; half of a stage's pieces go with either half's products
+  unsigned dp = d0 + (NST - 1) * SB;
+  for (int t = 0, s0 = 0, s1 = 1;;) {
+    half(0, t, s0, Int<P1>{}, Int<P>{}, dp);
+    end();
     tile::wait_vm<(NST - 2) * P>();                      // stage t + 1 has arrived
     if (t + 2 == nk) mend(s1);
-    tile::done_reading();
+    done();
     begin();
-    half(1, t + 1, s1, Int<1>{}, __builtin_amdgcn_readfirstlane(d0 + s0 * SB));
-    end();
+    dp = __builtin_amdgcn_readfirstlane(d0 + s0 * SB);
+    half(1, t + 1, s1, Int<0>{}, Int<P1>{}, dp);
     s0 = s1, s1 = s1 == NST - 1 ? 0 : s1 + 1;            // (the last step reads a slot that holds an earlier stage, or none: unused)
     if (++t == nk) break;
   }

@@ -13,23 +13,20 @@ using mx::TileArgs;
 
 namespace {
 
-template <int XR, int RT, int NW, int D, int KS>
+template <int XR, int RT, int NW, int D>
 struct Ring {
   static constexpr int MT = XR < 16 ? 1 : XR / 16;       // fragments of x (of fewer than 16 rows: read again, never stored)
-  static constexpr int NH = KS / 32;                     // products along a stage
-  static constexpr int XB = XR * KS * 2, XP = XB / 1024; // bytes and DMA pieces of x in a stage
-  static constexpr int WP = KS == 128 ? RT : (RT + 1) / 2, WB = WP * 1024;
-  static constexpr int SP = (RT + 3) / 4, SB = XB + WB + SP * 256, G = XP + WP + SP;
+  static constexpr int XB = XR * 256, XP = XB / 1024;    // bytes and DMA pieces of x in a stage
+  static constexpr int SP = (RT + 3) / 4, WB = RT * 1024, SB = XB + WB + SP * 256, G = XP + RT + SP;
   static constexpr int PART = RT * MT * 1024;            // a wave's sums
   static constexpr int LDS = NW * D * SB > NW * PART ? NW * D * SB : NW * PART;
   static_assert(XB % 1024 == 0 && LDS <= mx::kLds && D >= 2 && G * (D - 1) < 64, "ring");
 };
 
-template <typename T, int XR, int RT, int NW, int D, int KS>
+template <typename T, int XR, int RT, int NW, int D>
 __global__ void __launch_bounds__(64 * NW, 1) rows_kernel(const TileArgs a) {
-  using S = Ring<XR, RT, NW, D, KS>;
-  constexpr int MT = S::MT, XP = S::XP, WP = S::WP, SP = S::SP, NH = S::NH, XB = S::XB, WB = S::WB, G = S::G;
-  constexpr int CH = KS / 8, RP = 64 / CH;               // 16-byte chunks of a row of x in a stage; rows of a piece
+  using S = Ring<XR, RT, NW, D>;
+  constexpr int MT = S::MT, XP = S::XP, SP = S::SP, XB = S::XB, WB = S::WB, G = S::G;
   __shared__ __attribute__((aligned(16))) char lds[S::LDS];
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -38,41 +35,31 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_kernel(const TileArgs a) {
   const int m0 = tm * XR, n0 = tn * 16 * RT;
   char* ring = lds + wid * D * S::SB;
   const unsigned ring0 = __builtin_amdgcn_readfirstlane(mx::lds_addr(ring));
-  const int steps = (a.K + KS - 1) / KS, t0 = steps * wid / NW, nk = steps * (wid + 1) / NW - t0;
+  const int steps = (a.K + 127) / 128, t0 = steps * wid / NW, nk = steps * (wid + 1) / NW - t0;
   const char* xb = (const char*)a.x + (long long)m0 * a.ldx * 2;
   const long long wp = (long long)a.N * 64, sp = (long long)a.N * 4;
-  // a lane's place in the pieces; chunk c of row r of x lies at c ^ (r & 15) (KS 64: c ^ (r / 2 & 7))
-  unsigned offx[XP], offw[WP], offs[SP];
-  const int cx = KS == 128 ? (lane & 15) : (lane & 7), rx = lane / CH;
-  auto swz = [](int r) { return KS == 128 ? r & 15 : (r >> 1) & 7; };
+  // a lane's place in the pieces; chunk c of row r of x lies at c ^ (r & 15)
+  unsigned offx[XP], offw[RT], offs[SP];
+  auto chunk = [&](int q) { return (lane & 15) ^ ((4 * q + (lane >> 4)) & 15); };        // of x, that the lane brings with piece q
 #pragma unroll
-  for (int q = 0; q < XP; ++q) {
-    const int r = RP * q + rx;
-    offx[q] = (unsigned)min(r, a.M - m0 - 1) * (unsigned)(2 * a.ldx) + 16 * (cx ^ swz(r));
-  }
+  for (int q = 0; q < XP; ++q) offx[q] = (unsigned)min(4 * q + (lane >> 4), a.M - m0 - 1) * (unsigned)(2 * a.ldx) + 16 * chunk(q);
 #pragma unroll
-  for (int q = 0; q < WP; ++q)
-    offw[q] = KS == 128 ? (unsigned)min(n0 + 16 * q + (lane >> 2), a.N - 1) * 64u + 16 * (lane & 3)
-                        : (unsigned)min(n0 + 32 * q + (lane >> 1), a.N - 1) * 64u + 16 * ((lane ^ lane >> 4) & 1);
+  for (int q = 0; q < RT; ++q) offw[q] = (unsigned)min(n0 + 16 * q + (lane >> 2), a.N - 1) * 64u + 16 * (lane & 3);
 #pragma unroll
   for (int q = 0; q < SP; ++q) offs[q] = (unsigned)min(n0 + 64 * q + lane, a.N - 1) * 4u;
-  const int tail = a.K - KS * (steps - 1);               // values of x in the last stage
+  const int tail = a.K - 128 * (steps - 1);               // values of x in the last stage
   auto issue = [&](int i) __attribute__((always_inline)) {               // the wave's stage i
     const int t = t0 + i;
     const bool last = t == steps - 1;
     const unsigned d = ring0 + i % D * S::SB;
-    const char* xs = xb + (long long)t * (2 * KS);
-    const char* ws = KS == 128 ? (const char*)a.codes + t * wp : (const char*)a.codes + (t >> 1) * wp + (t & 1) * 32;
-    const char* ss = (const char*)a.scales + (KS == 128 ? t : t >> 1) * sp;
+    const char *xs = xb + (long long)t * 256, *ws = (const char*)a.codes + t * wp, *ss = (const char*)a.scales + t * sp;
 #pragma unroll
-    for (int q = 0; q < WP; ++q) tile::dma16(ws, offw[q], __builtin_amdgcn_readfirstlane(d + XB + q * 1024));
+    for (int q = 0; q < RT; ++q) tile::dma16(ws, offw[q], __builtin_amdgcn_readfirstlane(d + XB + q * 1024));
 #pragma unroll
     for (int q = 0; q < SP; ++q) mx::dma4(ss, offs[q], __builtin_amdgcn_readfirstlane(d + XB + WB + q * 256));
 #pragma unroll
-    for (int q = 0; q < XP; ++q) {
-      const int c = cx ^ swz(RP * q + rx);
-      tile::dma16(xs, offx[q] - (last && 8 * c >= tail ? 16 * c : 0), __builtin_amdgcn_readfirstlane(d + q * 1024));
-    }
+    for (int q = 0; q < XP; ++q)
+      tile::dma16(xs, offx[q] - (last && 8 * chunk(q) >= tail ? 16 * chunk(q) : 0), __builtin_amdgcn_readfirstlane(d + q * 1024));
   };
   f32x4 acc[RT][MT];
 #pragma unroll
@@ -90,37 +77,30 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_kernel(const TileArgs a) {
     asm volatile("" ::: "memory");
     char* img = ring + i % D * S::SB;
     const int t = t0 + i;
-    if (t == steps - 1 && tail < KS) {                   // what lies beyond k: zeros
+    if (t == steps - 1 && tail < 128) {                  // what lies beyond k: zeros
 #pragma unroll
       for (int q = 0; q < XP; ++q)
-        if (8 * (cx ^ swz(RP * q + rx)) >= tail) *reinterpret_cast<uint4*>(img + q * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
+        if (8 * chunk(q) >= tail) *reinterpret_cast<uint4*>(img + q * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
     }
-    unsigned sc[RT], raw[RT][NH];
+    float sc[RT];
+    uint4 raw[RT];
 #pragma unroll
-    for (int u = 0; u < RT; ++u) {
-      sc[u] = *reinterpret_cast<const unsigned*>(img + XB + WB + (16 * u + lr) * 4);
-      if constexpr (KS == 128) {                         // block lg of the lane's row
-        const uint4 v = *reinterpret_cast<const uint4*>(img + XB + u * 1024 + lr * 64 + lg * 16);
-        raw[u][0] = v.x, raw[u][1] = v.y, raw[u][NH - 2] = v.z, raw[u][NH - 1] = v.w;
-      } else {
-#pragma unroll
-        for (int h = 0; h < NH; ++h)
-          raw[u][h] = *reinterpret_cast<const unsigned*>(img + XB + u * 512 + lr * 32 + (((h ^ lr >> 3) & 1) << 4) + lg * 4);
-      }
+    for (int u = 0; u < RT; ++u) {                       // block lg of the lane's row and its scale
+      sc[u] = mx_scale_of(*reinterpret_cast<const unsigned*>(img + XB + WB + (16 * u + lr) * 4), 9 + 8 * lg);
+      raw[u] = *reinterpret_cast<const uint4*>(img + XB + u * 1024 + lr * 64 + lg * 16);
     }
-    // KS 128: lane (lr, lg) multiplies k 32 lg + 8 h .. + 7 in step h; 64: k 32 h + 8 lg ..
+    // lane (lr, lg) multiplies k 32 lg + 8 h .. + 7 in step h
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
+    for (int h = 0; h < 4; ++h) {
       uint4 b[MT];
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        const int r = (16 * j + lr) & (XR - 1), c = KS == 128 ? 4 * lg + h : 4 * h + lg;
-        b[j] = *reinterpret_cast<const uint4*>(img + r * (2 * KS) + ((c ^ swz(r)) << 4));
+        const int r = (16 * j + lr) & (XR - 1);
+        b[j] = *reinterpret_cast<const uint4*>(img + r * 256 + (((4 * lg + h) ^ (r & 15)) << 4));
       }
 #pragma unroll
       for (int u = 0; u < RT; ++u) {
-        const int byte = KS == 128 ? lg : 2 * (t & 1) + h;
-        const uint4 w = unfold<T>(raw[u][h], mx_scale((sc[u] >> (8 * byte)) & 255u));
+        const uint4 w = unfold<T>(h == 0 ? raw[u].x : h == 1 ? raw[u].y : h == 2 ? raw[u].z : raw[u].w, sc[u]);
 #pragma unroll
         for (int j = 0; j < MT; ++j) acc[u][j] = Mfma<T>::run(w, b[j], acc[u][j]);
       }
@@ -142,6 +122,56 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_kernel(const TileArgs a) {
   }
 }
 
+// The same on mx_loop.h's loop: the wave's stages are 64 k, and reads, conversions and DMA stand between its products.
+template <typename T, int RT, int MT>
+__global__ void __launch_bounds__(256, 1) rows_loop_kernel(const TileArgs a) {
+  using S = mx::Shape<RT, MT, -4, false>;
+  constexpr int NW = 4, XR = 16 * MT, PART = RT * MT * 1024;
+  __shared__ __attribute__((aligned(16))) char lds[NW * (S::LDS > PART ? S::LDS : PART)];
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = tile::unit_of(blockIdx.x, gridDim.x);
+  const int tm = tile % a.tiles_m, tn = tile / a.tiles_m;                // the row groups of a column tile share an XCD
+  const int m0 = tm * XR, n0 = tn * 16 * RT;
+  const int steps = (a.K + 63) / 64, t0 = steps * wid / NW, nk = steps * (wid + 1) / NW - t0;
+  const long long wp = (long long)a.N * 64, sp = (long long)a.N * 4;
+  f32x4 acc[RT][MT];
+  if (nk > 0) {
+    unsigned offx[S::PX], offw[S::PW], offs[S::PS];
+#pragma unroll
+    for (int q = 0; q < S::PX; ++q) {
+      const int r = 8 * q + (lane >> 3);
+      offx[q] = (unsigned)min(r, a.M - m0 - 1) * (unsigned)(2 * a.ldx) + 16 * ((lane & 7) ^ tile::swz(r));
+    }
+#pragma unroll
+    for (int q = 0; q < S::PW; ++q) offw[q] = (unsigned)min(n0 + 32 * q + (lane >> 1), a.N - 1) * 64u + 16 * ((lane ^ lane >> 4) & 1);
+#pragma unroll
+    for (int q = 0; q < S::PS; ++q) offs[q] = (unsigned)min(n0 + 64 * q + lane, a.N - 1) * 4u;
+    const mx::Walk walk{(const char*)a.x + (long long)m0 * a.ldx * 2 + (long long)t0 * 128, (const char*)a.codes + (t0 >> 1) * wp + (t0 & 1) * 32,
+                        (const char*)a.scales + (t0 >> 1) * sp, wp, sp, nk, t0 + nk == steps ? a.K - 64 * (steps - 1) : 64, 64, t0 & 1};
+    mx::products<T, RT, MT, -4, false>(lds + wid * S::LDS, walk, offx, offw, offs, offw, offs, acc);
+  } else {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // the waves' sums, over the rings
+  tile::done_reading();
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(lds + wid * PART + (i * MT + j) * 1024 + lane * 16) = acc[i][j];
+  __syncthreads();
+  for (int q = wid; q < RT * MT; q += NW) {
+    f32x4 v = *reinterpret_cast<const f32x4*>(lds + q * 1024 + lane * 16);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const f32x4*>(lds + w * PART + q * 1024 + lane * 16);
+    const int i = q / MT, m = m0 + 16 * (q - i * MT) + lr;
+    if (m < a.M) mx::put<T>(a, m, n0 + 16 * i + 4 * lg, false, v, v);
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -156,15 +186,21 @@ hipError_t sm_mx_rows(int dt, const void* x, long long ldx, const void* codes, c
   int grid;
   if (!mx::plan(a, N, xr, 16 * rt, grid)) return hipErrorInvalidValue;
   switch (10 * xr + rt) {
-#define GO(XR, RT, NW, D, KS)                                                                  \
-  case 10 * XR + RT:                                                                           \
-    if (dt == kBF16) rows_kernel<bf16, XR, RT, NW, D, KS><<<grid, 64 * NW, 0, st>>>(a);        \
-    else rows_kernel<fp16, XR, RT, NW, D, KS><<<grid, 64 * NW, 0, st>>>(a);                    \
+#define GO(XR, RT, NW, D)                                                                \
+  case 10 * XR + RT:                                                                     \
+    if (dt == kBF16) rows_kernel<bf16, XR, RT, NW, D><<<grid, 64 * NW, 0, st>>>(a);      \
+    else rows_kernel<fp16, XR, RT, NW, D><<<grid, 64 * NW, 0, st>>>(a);                  \
     break;
-    GO(4, 1, 8, 8, 128) GO(4, 2, 8, 6, 128) GO(4, 3, 8, 4, 128) GO(4, 4, 8, 3, 128) GO(4, 6, 8, 2, 128) GO(4, 8, 4, 4, 128)
-    GO(16, 1, 8, 3, 128) GO(16, 2, 8, 3, 128) GO(16, 3, 8, 2, 128) GO(16, 4, 8, 2, 128) GO(16, 6, 4, 3, 128) GO(16, 8, 4, 3, 128)
-    GO(32, 1, 4, 4, 128) GO(32, 2, 4, 3, 128) GO(32, 3, 4, 3, 128) GO(32, 4, 4, 3, 128) GO(32, 6, 4, 2, 128) GO(32, 8, 4, 4, 64)
-    GO(64, 1, 4, 4, 64) GO(64, 2, 4, 4, 64) GO(64, 3, 4, 3, 64) GO(64, 4, 4, 3, 64) GO(64, 6, 4, 3, 64) GO(64, 8, 4, 3, 64)
+    GO(4, 1, 8, 8) GO(4, 2, 8, 6) GO(4, 3, 8, 4) GO(4, 4, 8, 3) GO(4, 6, 8, 2) GO(4, 8, 4, 4)
+    GO(16, 1, 8, 3) GO(16, 2, 8, 3) GO(16, 3, 8, 2) GO(16, 4, 8, 2) GO(16, 6, 4, 3) GO(16, 8, 4, 3)
+    GO(32, 1, 4, 4) GO(32, 2, 4, 3) GO(32, 3, 4, 3) GO(32, 4, 4, 3) GO(32, 6, 4, 2)
+#undef GO
+#define GO(XR, RT)                                                                       \
+  case 10 * XR + RT:                                                                     \
+    if (dt == kBF16) rows_loop_kernel<bf16, RT, XR / 16><<<grid, 256, 0, st>>>(a);       \
+    else rows_loop_kernel<fp16, RT, XR / 16><<<grid, 256, 0, st>>>(a);                   \
+    break;
+    GO(32, 8) GO(64, 1) GO(64, 2) GO(64, 3) GO(64, 4) GO(64, 6) GO(64, 8)
 #undef GO
     default: return hipErrorInvalidValue;
   }
