@@ -197,14 +197,14 @@ def _decode(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return (v * _power(scales).unsqueeze(-1)).reshape(R, n * BLOCK)[:, :K]
 
 
-# What a round of 256 workgroups takes, us (bf16, weights from HBM): (a + b rt) a stage of 64 k and (f + g rt) beside them on the
-# few-row kernel's xr x 16 rt results, c and e on tiles of 32 mj x 32 ni.  Measured with one round: 64 x 16 results at K = 4096 / 11008 11.4 /
-# 26, 64 x 128 23 / 51, 32 x 16 7.9 / 16, 16 x 16 5.8 / 10.8, 4 x 16 4.8 / 8.3; 256 x 128 64 / 171, 256 x 256 107 / 267.  Up to some 500
-# rows the few-row kernel's small results fill the chip (509 x 4096 x 4096 33 -> 23 us), beyond them tiles read x fewer times.
+# What a round of 256 workgroups takes, us (bf16, weights from HBM), as a time a stage of 64 k and one beside them: a + b rt and f + g rt on the
+# few-row kernel's xr x 16 rt results, c and e on tiles of 32 mj x 32 ni.
 _ROWS = [(xr, 16 * rt, (0, xr, rt), a + b * rt, f + g * rt)
-         for xr, a, b, f, g in ((4, 0.026, 0.0062, 2.5, 0.2), (16, 0.035, 0.0105, 2.8, 0.1), (32, 0.063, 0.0155, 2.8, 0.15), (64, 0.118, 0.0187, 2.2, 0.43))
-         for rt in (1, 2, 3, 4, 6, 8)]
-_TILES = [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.95, 6.0), (6, 1.15, 7.0), (8, 1.48, 12.0))]
+         for xr, a, b, f, g, rts in ((4, 0.02, 0.008, 2.0, 0.4, (1, 2, 3, 4, 6, 8)), (16, 0.03, 0.0075, 1.9, 0.5, (1, 2, 3, 4, 6, 8)),
+                                     (32, 0.075, 0.0135, 1.5, 0.5, (1, 2, 3, 4, 6)), (32, 0.24, 0.0, 5.9, 0.0, (8,)),
+                                     (64, 0.1, 0.02, 2.0, 0.6, (1, 2, 3, 4, 6, 8)))
+         for rt in rts]
+_TILES = [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.75, 10.0), (6, 1.03, 11.5), (8, 1.25, 14.5))]
 
 
 def _best(M: int, N: int, K: int, forms) -> tuple:
@@ -223,7 +223,7 @@ _MATMUL = ([(xr, 16 * rt, (0, xr, rt), (a + b * rt) / 2, f + g * rt)
             for xr, a, b, f, g, rts in ((16, 0.05, 0.0125, 2.9, 0.1, (1, 2, 4, 6, 8)), (32, 0.05, 0.015, 3.3, 0.1, (1, 2, 4, 6, 8)),
                                         (64, 0.087, 0.013, 2.8, 0.4, (1, 2, 3, 4, 6, 8)), (128, 0.0, 0.048, 0.0, 1.4, (4,)))
             for rt in rts]
-           + [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.36, 10.0), (6, 0.43, 12.0), (8, 0.515, 15.7))])
+           + [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.27, 11.5), (6, 0.34, 12.0), (8, 0.40, 14.5))])
 
 
 @functools.lru_cache(4096)
@@ -234,8 +234,8 @@ def _matmul_form(M: int, N: int, K: int) -> tuple:
 
 # the gradient likewise, a stage 64 of the weight's rows (4096 / 12288 of them: 64 x 128 results 24 / 60, 32 x 128 17 / 42, 16 x 128 13 / 30; 128 x
 # 256 72 / 200; 509 x 4096 x 4096 on 64 x 128 26, on 64 x 256 tiles 48)
-_GRAD = ([(xr, 128, (0, xr, 0), c, e) for xr, c, e in ((16, 0.133, 4.8), (32, 0.2, 4.2), (64, 0.28, 6.5))]
-         + [(32 * mj, 256, (1, mj, 2), c, e) for mj, c, e in ((4, 1.0, 6.0), (8, 1.42, 8.0))])
+_GRAD = ([(xr, 128, (0, xr, 0), c, e) for xr, c, e in ((16, 0.15, 4.5), (32, 0.21, 4.6), (64, 0.28, 5.4))]
+         + [(32 * mj, 256, (1, mj, 2), c, e) for mj, c, e in ((4, 0.83, 11.5), (8, 1.4, 13.0))])
 
 
 @functools.lru_cache(4096)
