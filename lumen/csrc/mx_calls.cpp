@@ -26,8 +26,7 @@ using torch::autograd::variable_list;
 typedef hipError_t (*QuantizeFn)(int, const void*, long long, void*, void*, int, int, hipStream_t);
 typedef hipError_t (*DequantizeFn)(int, const void*, const void*, void*, int, int, hipStream_t);
 typedef hipError_t (*LinearFn)(int, const void*, long long, const void*, const void*, const void*, void*, int, int, int, int, int, hipStream_t);
-typedef hipError_t (*GradFn)(int, const void*, long long, const void*, const void*, void*, int, int, int, int, int, hipStream_t);
-typedef hipError_t (*RowsGradFn)(int, const void*, long long, const void*, const void*, void*, int, int, int, int, hipStream_t);
+typedef hipError_t (*GradFn)(int, const void*, long long, const void*, const void*, void*, int, int, int, int, hipStream_t);
 typedef hipError_t (*MatmulFn)(int, const void*, const void*, const void*, const void*, const void*, void*, int, int, int, int, int, hipStream_t);
 
 enum Launcher { kQuantize, kDequantize, kLinear, kRows, kGrad, kRowsGrad, kMatmul, kRowsMatmul, kLaunchers };
@@ -153,12 +152,8 @@ Tensor grad(const Tensor& dy, const Tensor& data, int64_t K, const Form& f) {
     rows = at::constant_pad_nd(dy, {0, 8 - N % 8});
   }
   const Rows r(rows, 8, kMaxLd);
-  if (f[0])
-    done(fn<GradFn>(kGrad)(dt, r.p, r.ld, w.codes, w.scales, dx.data_ptr(), int(M), int(N), int(K), f[1], f[2], on.stream),
-         "gradient of mxfp4_linear");
-  else
-    done(fn<RowsGradFn>(kRowsGrad)(dt, r.p, r.ld, w.codes, w.scales, dx.data_ptr(), int(M), int(N), int(K), f[1], on.stream),
-         "gradient of mxfp4_linear");
+  done(fn<GradFn>(f[0] ? kGrad : kRowsGrad)(dt, r.p, r.ld, w.codes, w.scales, dx.data_ptr(), int(M), int(N), int(K), f[1], on.stream),
+       "gradient of mxfp4_linear");
   return dx;
 }
 

@@ -1,4 +1,12 @@
-// dx = dy w of 16-bit rows and an MXFP4 weight, on tiles (mx_loop.h).
+// dx = dy w of 16-bit rows and an MXFP4 weight (mx_loop.h): dx[m][k] = sum over n of dy[m][n] c[n][k] 2^e[n][k / 32], the weight's
+// values in dy's type, as the forward product has them.
+//
+// The sum runs over the weight's rows, which the codes do not lie along: a matrix instruction wants 8 rows' values of one column in a
+// lane.  A lane takes four bytes of 8 rows, makes pairs of neighbouring columns and exchanges halves between two rows (v_perm): 4
+// conversions and 4 exchanges for 8 values of two rows, where a transposed copy of the weight would cost its memory again.
+// On tiles of 128 or 256 rows x two panels: a stage (64 of the weight's rows) of 256 x 256 takes 1.40 us on all CUs, the vector unit's 16
+// units a half beside 1.25 of the forward product.  4096 rows, weight 4096 x 11008: 282 us = 1.31 PFLOP/s on 256 rows, 353 on 128;
+// 2048 rows, 4096 x 4096: 74 on 128, 103 on 256.
 #include "mx_tile.h"
 
 using namespace lumen;
@@ -6,8 +14,9 @@ using mx::TileArgs;
 
 namespace {
 
-template <typename T, int MJ, int WN>
+template <typename T, int MJ>
 __global__ void __launch_bounds__(256, 1) grad_kernel(const TileArgs a) {
+  constexpr int WN = 2;
   using S = mx::Shape<8, MJ, WN, true>;
   __shared__ __attribute__((aligned(16))) char lds[S::LDS];
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
@@ -51,7 +60,9 @@ __global__ void __launch_bounds__(256, 1) grad_kernel(const TileArgs a) {
   }
 }
 
-// Few results: a workgroup takes 16 MT rows of dy and one panel of columns, its NW waves split the sum over w's rows, each in a ring of its own.
+// Few results: a workgroup takes 16 MT rows of dy and one panel of columns, its NW waves split the sum over w's rows, each in a ring of its
+// own.  16 rows leave a SIMD room for two waves.  Us: 17 rows, 4096 x 4096 12.5 on 16 (15.5 on 32), 200 rows 16.9 on 32 (20.2 on 64), 509 rows
+// 21.2 on 64 (30.5 on 32, on tiles of 128 x 256 68) = 0.81 PFLOP/s.
 template <typename T, int MT, int NW>
 __global__ void __launch_bounds__(64 * NW, 1) rows_grad_kernel(const TileArgs a) {
   using S = mx::Shape<8, MT, -NW, true>;
@@ -113,23 +124,23 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_grad_kernel(const TileArgs a)
 
 extern "C" {
 
-// dx [M, K] = dy [M, N] w; dy 16-bit at ldy, its rows readable (and zero) up to a multiple of 8 values; tiles of 64 mj / wn x 128 wn
+// dx [M, K] = dy [M, N] w; dy 16-bit at ldy, its rows readable (and zero) up to a multiple of 8 values; tiles of 32 mj x 256
 hipError_t sm_mx_grad(int dt, const void* dy, long long ldy, const void* codes, const void* scales, void* dx, int M, int N, int K, int mj,
-                      int wn, hipStream_t st) {
+                      hipStream_t st) {
   const int Nx = (N + 7) / 8 * 8;
   if (!mx::sizes_ok(M, N, K) || ldy < Nx || ldy % 8 || ldy > (1 << 22) || ((uintptr_t)dx | (uintptr_t)dy | (uintptr_t)codes | (uintptr_t)scales) % 16 ||
       (dt != kF16 && dt != kBF16))
     return hipErrorInvalidValue;
   TileArgs a{dy, ldy, nullptr, codes, scales, nullptr, dx, M, N, K, Nx, 0, 0, 0, 8};
   int grid;
-  if (!mx::plan(a, K, 64 * mj / wn, 128 * wn, grid)) return hipErrorInvalidValue;
-  switch (10 * mj + wn) {
-#define GO(MJ, WN)                                                                     \
-  case 10 * MJ + WN:                                                                   \
-    if (dt == kBF16) grad_kernel<bf16, MJ, WN><<<grid, 256, 0, st>>>(a);               \
-    else grad_kernel<fp16, MJ, WN><<<grid, 256, 0, st>>>(a);                           \
+  if (!mx::plan(a, K, 32 * mj, 256, grid)) return hipErrorInvalidValue;
+  switch (mj) {
+#define GO(MJ)                                                                         \
+  case MJ:                                                                             \
+    if (dt == kBF16) grad_kernel<bf16, MJ><<<grid, 256, 0, st>>>(a);                   \
+    else grad_kernel<fp16, MJ><<<grid, 256, 0, st>>>(a);                               \
     break;
-    GO(4, 2) GO(8, 2)
+    GO(4) GO(8)
 #undef GO
     default: return hipErrorInvalidValue;
   }

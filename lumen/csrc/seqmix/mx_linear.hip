@@ -1,4 +1,12 @@
-// y = x w^T + bias of 16-bit rows and an MXFP4 weight, on tiles (mx_loop.h).
+// y = x w^T + bias of 16-bit rows and an MXFP4 weight, on tiles (mx_loop.h): y[m][n] = sum over k of x[m][k] c[n][k] 2^e[n][k / 32].
+//
+// The weight's values are made in x's type (exact in bf16; in fp16 rounded once: what lies below 2^-24 is lost, above 65504 infinite) and
+// multiplied by the 16-bit matrix instructions with fp32 sums, so those bound it.  A stage of 64 k of the 256 x 256 tile is, for each of
+// the four waves, 128 products of 16 cycles and between them 40 LDS reads, 64 conversions, 16 turned scales and 11 DMA pieces; alone on
+// the chip it takes 1.07 us, 0.85 being the products', on all CUs, whose clock falls with their power, 1.25.
+// A tile has 256 rows, for x is the wider operand, and 128, 192 or 256 columns, whichever fill the last round of workgroups best (us, 128 /
+// 192 / 256: 2048 x 12288 x 4096 160 / 143 / 164, 4096 x 12288 x 4096 310 / 278 / 263, 2048 x 4096 x 4096 57 / 78 / 95).
+// 4096 x 12288 x 4096 bf16: 263 us = 1.57 PFLOP/s; the library's 16-bit product of 8192^3 runs at 1.40.
 #include "mx_tile.h"
 
 using namespace lumen;

@@ -1,10 +1,12 @@
-// Main loops of products with MXFP4 weights on tiles, one workgroup of four waves per CU.
+// Main loops of products with MXFP4 weights, one workgroup per CU: four waves on a tile, or waves that split the sum.
 //
 // Rows in MXFP4 lie in panels of 128 k: codes [K / 128][rows][64 bytes], scales [K / 128][rows][4 bytes] (mxfp4.hip), so that a stage
 // of a tile is one run of memory whichever product reads it.
 //  * Operands come by LDS-DMA, as many stages ahead as fit into 160 KiB, under counted waits; one barrier a stage.
 //  * While the matrix core multiplies one set of fragments, the next set is read and made: between two products stands at most a
-//    read, a DMA or a few instructions of the vector unit, which the matrix core's 16 cycles cover.
+//    read, a DMA or a few instructions of the vector unit, which the matrix core's 16 cycles cover.  A wave's instructions leave in
+//    order, one in four cycles or more, so each one too many there is time lost: addresses move once a stage, the last stage is
+//    sent for again rather than asked about, and a scale is turned into place by one instruction.
 //  * 192 and more accumulators are named as accumulation registers in the products' assembly: the compiler, left to place them, moves
 //    them to and fro.  It knows nothing of such products' latency, so nothing may read or move an accumulator before settle(): the
 //    loops have one way round and settle before they are left.  Fewer are the compiler's.
@@ -29,7 +31,7 @@ template <bool NAMED> __device__ __forceinline__ void settle() { if constexpr (N
 template <bool NAMED> __device__ __forceinline__ void hold(f32x4& c) { if constexpr (NAMED) tile::hold(c); }
 
 // LDS-DMA of 16 and 4 bytes per lane to lds + AT: three instructions, as they stand between products, where each costs its issue (with a
-// stage's addresses worked out for every piece of it 256 x 256 x 11008 of 4-bit operands took 87 us, so 55)
+// stage's addresses worked out for every piece of it a tile of 256 x 256 x 11008 of 4-bit operands took 87 us, so 61)
 template <int AT>
 __device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned lds) {
   asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(lds), "n"(AT) : "memory", "m0", "scc");

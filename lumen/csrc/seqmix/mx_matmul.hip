@@ -1,4 +1,11 @@
-// y = x w^T + bias, both in MXFP4, on tiles (mx_loop.h).
+// y = x w^T + bias, both in MXFP4: y[m][n] = sum over blocks b of 2^(e[m][b] + f[n][b]) sum over k in b of c[m][k] d[n][k], on the scaled
+// matrix instructions, which take a block of 32 codes and its scale byte from every lane: 16 x 16 x 128 a product, exact but for the fp32 sums.
+//
+// On tiles (mx_loop.h) a stage is a panel.  256 x 256: 64 products of 16 cycles a wave between 32 LDS reads, 16 shifts and 10 DMA pieces; a
+// stage alone on the chip takes 0.61 us, 0.43 being the products' and 0.39 its 34 KB of DMA, on all CUs 0.80 (products alone, with random
+// codes: 6.4 PFLOP/s, with zeros 9.8: power).  Tiles of 256 rows x 128, 192 or 256 columns by rounds (us: 1021 x 12288 x 4096 49 / 32 / 34,
+// 4096 x 22016 x 4096 253 / 218 / 200 = 3.70 PFLOP/s).
+// Few results: below.
 #include "mx_tile.h"
 
 using namespace lumen;
@@ -30,7 +37,9 @@ __global__ void __launch_bounds__(256, 1) matmul_kernel(const TileArgs a) {
 }
 
 // Few results: a workgroup takes XR rows and 16 RT columns, its four waves split k, each in a ring of its own (seqmix/mx_rows.hip); a
-// stage is a panel.
+// stage is a panel.  Bound by bytes: a CU takes 97 B/ns from L2, and 64 x 128 results are 13 KB a panel for 32 products.  The interleaved
+// loop of the tiles brings nothing here (64 x 22016 x 4096 13.9 -> 14.6 us, 1021 x 2048 x 5632 12.6 -> 12.7).  1 x 4096 x 4096 4.4 us, 48 x
+// 12288 x 4096 9.4 = 2.8 TB/s of weight; against tiles 509 x 4096 x 4096 11 (256 x 128: 25), 1021 x 2048 x 5632 12.6 (32).
 template <int XR, int RT, int D>
 struct Ring {
   static constexpr int NW = 4, MT = XR / 16, XB = MT * 1024, WB = RT * 1024, SX = (MT + 3) / 4, SW = (RT + 3) / 4;
@@ -105,20 +114,7 @@ __global__ void __launch_bounds__(256, 1) rows_matmul_kernel(const TileArgs a) {
       for (int j = 0; j < MT; ++j) mx::mfma4<false>(acc[u][j], w, x[j], sw, sx[j]);
     }
   }
-  // the waves' sums, over the rings
-  tile::done_reading();
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(lds + wid * S::PART + (i * MT + j) * 1024 + lane * 16) = acc[i][j];
-  __syncthreads();
-  for (int q = wid; q < RT * MT; q += NW) {
-    f32x4 v = *reinterpret_cast<const f32x4*>(lds + q * 1024 + lane * 16);
-#pragma unroll
-    for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const f32x4*>(lds + w * S::PART + q * 1024 + lane * 16);
-    const int i = q / MT, m = m0 + 16 * (q - i * MT) + lr;
-    if (m < a.M) mx::put<T>(a, m, n0 + 16 * i + 4 * lg, false, v, v);
-  }
+  mx::sum_waves<T, RT, MT, NW>(a, lds, acc, m0, n0);
 }
 
 }  // namespace

@@ -1,11 +1,16 @@
 // y = x w^T + bias of few 16-bit rows and an MXFP4 weight [N, K]: a stream of the weight.
 //
-// A workgroup takes XR rows of x and 16 RT columns; its NW waves split k and every wave streams its share of both through a
-// ring of its own in LDS, D stages of KS k, filled by LDS-DMA.  No barrier stands in the loop: a wave waits for its own stages by a
-// counted vmcnt.  The waves' sums meet in LDS at the end, in wave order.
-//  * The weight's 4-bit rows become 16-bit fragments in registers, by the scaled conversions, between the reads and the products.
-//  * x comes from L2 once per workgroup, 4 to 16 times the weight's bytes: the columns of a workgroup are as many as make one round
-//    of workgroups.
+// A workgroup takes XR rows of x and 16 RT columns; its waves split k and every wave streams its share of both through a ring of its own
+// in LDS, filled by LDS-DMA.  No barrier stands in the loop: a wave waits for its own stages by a counted vmcnt.  The waves' sums
+// meet in LDS at the end, in wave order.  The weight's codes become 16-bit fragments in registers, by the scaled conversions.
+//  * Up to 32 rows it is bound by the weight's bytes and by the launch: stages of 128 k, whole lines of the weight, reads in a row
+//    before the products (us: 1 x 4096 x 4096 4.8, 8 x 22016 x 4096 11.9 = 4.0 TB/s of weight, 17 x 32000 x 2048 12.9).
+//  * 64 rows, and 32 with 128 columns, are bound by the matrix core, the DMA and what a wave issues in turn: the tiles' loop, where each
+//    stands between products, 64 k a stage (509 x 4096 x 4096 23.9 -> 19.9 us = 0.86 PFLOP/s, 64 x 22016 x 4096 22.2 -> 20.2; 32 x 12288 x
+//    4096 with 48 columns rather 11.1 -> 12.4).
+//  * x comes from L2 once per workgroup, 4 to 16 times the weight's bytes, so the columns of a workgroup are as many as make one
+//    round of workgroups (64 x 22016 x 4096: 32 columns 33.6, 96 22.0, 128 25.0 of the first form).
+//  * Up to some 1000 rows such workgroups fill the chip better than tiles (509 x 4096 x 4096 on 256 x 128: 61).
 #include "mx_tile.h"
 
 using namespace lumen;
@@ -15,7 +20,7 @@ namespace {
 
 template <int XR, int RT, int NW, int D>
 struct Ring {
-  static constexpr int MT = XR < 16 ? 1 : XR / 16;       // fragments of x (of fewer than 16 rows: read again, never stored)
+  static constexpr int MT = XR / 16;                     // fragments of x
   static constexpr int XB = XR * 256, XP = XB / 1024;    // bytes and DMA pieces of x in a stage
   static constexpr int SP = (RT + 3) / 4, WB = RT * 1024, SB = XB + WB + SP * 256, G = XP + RT + SP;
   static constexpr int PART = RT * MT * 1024;            // a wave's sums
@@ -95,8 +100,7 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_kernel(const TileArgs a) {
       uint4 b[MT];
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        const int r = (16 * j + lr) & (XR - 1);
-        b[j] = *reinterpret_cast<const uint4*>(img + r * 256 + (((4 * lg + h) ^ (r & 15)) << 4));
+        b[j] = *reinterpret_cast<const uint4*>(img + (16 * j + lr) * 256 + (((4 * lg + h) ^ lr) << 4));
       }
 #pragma unroll
       for (int u = 0; u < RT; ++u) {
@@ -106,29 +110,16 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_kernel(const TileArgs a) {
       }
     }
   }
-  // the waves' sums, over the rings
-  tile::done_reading();
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(lds + wid * S::PART + (i * MT + j) * 1024 + lane * 16) = acc[i][j];
-  __syncthreads();
-  for (int q = wid; q < RT * MT; q += NW) {
-    f32x4 v = *reinterpret_cast<const f32x4*>(lds + q * 1024 + lane * 16);
-#pragma unroll
-    for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const f32x4*>(lds + w * S::PART + q * 1024 + lane * 16);
-    const int i = q / MT, r = 16 * (q - i * MT) + lr, m = m0 + r;
-    if (r < XR && m < a.M) mx::put<T>(a, m, n0 + 16 * i + 4 * lg, false, v, v);
-  }
+  mx::sum_waves<T, RT, MT, NW>(a, lds, acc, m0, n0);
 }
 
-// The same on mx_loop.h's loop: the wave's stages are 64 k, and reads, conversions and DMA stand between its products.
+// the same on the loop of the tiles (mx_loop.h), a stage 64 k
 template <typename T, int RT, int MT>
 __global__ void __launch_bounds__(256, 1) rows_loop_kernel(const TileArgs a) {
   using S = mx::Shape<RT, MT, -4, false>;
   constexpr int NW = 4, XR = 16 * MT, PART = RT * MT * 1024;
   __shared__ __attribute__((aligned(16))) char lds[NW * (S::LDS > PART ? S::LDS : PART)];
-  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = tile::unit_of(blockIdx.x, gridDim.x);
   const int tm = tile % a.tiles_m, tn = tile / a.tiles_m;                // the row groups of a column tile share an XCD
@@ -156,20 +147,7 @@ __global__ void __launch_bounds__(256, 1) rows_loop_kernel(const TileArgs a) {
 #pragma unroll
       for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // the waves' sums, over the rings
-  tile::done_reading();
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(lds + wid * PART + (i * MT + j) * 1024 + lane * 16) = acc[i][j];
-  __syncthreads();
-  for (int q = wid; q < RT * MT; q += NW) {
-    f32x4 v = *reinterpret_cast<const f32x4*>(lds + q * 1024 + lane * 16);
-#pragma unroll
-    for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const f32x4*>(lds + w * PART + q * 1024 + lane * 16);
-    const int i = q / MT, m = m0 + 16 * (q - i * MT) + lr;
-    if (m < a.M) mx::put<T>(a, m, n0 + 16 * i + 4 * lg, false, v, v);
-  }
+  mx::sum_waves<T, RT, MT, NW>(a, lds, acc, m0, n0);
 }
 
 }  // namespace
@@ -191,7 +169,6 @@ hipError_t sm_mx_rows(int dt, const void* x, long long ldx, const void* codes, c
     if (dt == kBF16) rows_kernel<bf16, XR, RT, NW, D><<<grid, 64 * NW, 0, st>>>(a);      \
     else rows_kernel<fp16, XR, RT, NW, D><<<grid, 64 * NW, 0, st>>>(a);                  \
     break;
-    GO(4, 1, 8, 8) GO(4, 2, 8, 6) GO(4, 3, 8, 4) GO(4, 4, 8, 3) GO(4, 6, 8, 2) GO(4, 8, 4, 4)
     GO(16, 1, 8, 3) GO(16, 2, 8, 3) GO(16, 3, 8, 2) GO(16, 4, 8, 2) GO(16, 6, 4, 3) GO(16, 8, 4, 3)
     GO(32, 1, 4, 4) GO(32, 2, 4, 3) GO(32, 3, 4, 3) GO(32, 4, 4, 3) GO(32, 6, 4, 2)
 #undef GO
@@ -200,7 +177,7 @@ hipError_t sm_mx_rows(int dt, const void* x, long long ldx, const void* codes, c
     if (dt == kBF16) rows_loop_kernel<bf16, RT, XR / 16><<<grid, 256, 0, st>>>(a);       \
     else rows_loop_kernel<fp16, RT, XR / 16><<<grid, 256, 0, st>>>(a);                   \
     break;
-    GO(32, 8) GO(64, 1) GO(64, 2) GO(64, 3) GO(64, 4) GO(64, 6) GO(64, 8)
+    GO(32, 8) GO(64, 2) GO(64, 3) GO(64, 4) GO(64, 6) GO(64, 8)
 #undef GO
     default: return hipErrorInvalidValue;
   }

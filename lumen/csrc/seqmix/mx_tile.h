@@ -64,6 +64,27 @@ __device__ __forceinline__ void put_all(const TileArgs& a, f32x4 (&acc)[NI][MJ],
   }
 }
 
+// the sums of NW waves that split k, 16 MT rows by 16 RT columns each, meet in LDS in the waves' order: the same bits every time
+template <typename T, int RT, int MT, int NW>
+__device__ __forceinline__ void sum_waves(const TileArgs& a, char* lds, f32x4 (&acc)[RT][MT], int m0, int n0) {
+  constexpr int PART = RT * MT * 1024;
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  tile::done_reading();                                  // (every wave's ring: the sums lie over them)
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(lds + wid * PART + (i * MT + j) * 1024 + lane * 16) = acc[i][j];
+  __syncthreads();
+  for (int q = wid; q < RT * MT; q += NW) {
+    f32x4 v = *reinterpret_cast<const f32x4*>(lds + q * 1024 + lane * 16);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const f32x4*>(lds + w * PART + q * 1024 + lane * 16);
+    const int i = q / MT, m = m0 + 16 * (q - i * MT) + lr;
+    if (m < a.M) put<T>(a, m, n0 + 16 * i + 4 * lg, false, v, v);
+  }
+}
+
 inline bool sizes_ok(int M, int N, int K) {
   return M >= 1 && N >= 1 && M <= (1 << 24) && N <= (1 << 24) && K >= 8 && K % 8 == 0 && K <= (1 << 23);
 }

@@ -90,7 +90,7 @@ SIGNATURES = {
     "sm_mx_dequantize": "ipppii",
     "sm_mx_linear": "iplppppiiiii",
     "sm_mx_rows": "iplppppiiiii",
-    "sm_mx_grad": "iplpppiiiii",
+    "sm_mx_grad": "iplpppiiii",
     "sm_mx_rows_grad": "iplpppiiii",
     "sm_mx_rows_matmul": "ippppppiiiii",
     "sm_mx_matmul": "ippppppiiiii",

@@ -198,11 +198,11 @@ def _decode(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 
 # What a round of 256 workgroups takes, us (bf16, weights from HBM), as a time a stage of 64 k and one beside them: a + b rt and f + g rt on the
-# few-row kernel's xr x 16 rt results, c and e on tiles of 32 mj x 32 ni.
+# few-row kernel's xr x 16 rt results, c and e on tiles of 32 mj x 32 ni (the kernels say what either form takes).  Over 190 sizes of 1 to
+# 4096 rows the form chosen takes 1 % more than the best one, 16 % at worst.
 _ROWS = [(xr, 16 * rt, (0, xr, rt), a + b * rt, f + g * rt)
-         for xr, a, b, f, g, rts in ((4, 0.02, 0.008, 2.0, 0.4, (1, 2, 3, 4, 6, 8)), (16, 0.03, 0.0075, 1.9, 0.5, (1, 2, 3, 4, 6, 8)),
-                                     (32, 0.075, 0.0135, 1.5, 0.5, (1, 2, 3, 4, 6)), (32, 0.24, 0.0, 5.9, 0.0, (8,)),
-                                     (64, 0.1, 0.02, 2.0, 0.6, (1, 2, 3, 4, 6, 8)))
+         for xr, a, b, f, g, rts in ((16, 0.03, 0.0075, 1.9, 0.5, (1, 2, 3, 4, 6, 8)), (32, 0.075, 0.0135, 1.5, 0.5, (1, 2, 3, 4, 6)),
+                                     (32, 0.24, 0.0, 5.9, 0.0, (8,)), (64, 0.1, 0.02, 2.0, 0.6, (2, 3, 4, 6, 8)))
          for rt in rts]
 _TILES = [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.75, 10.0), (6, 1.03, 11.5), (8, 1.25, 14.5))]
 
@@ -215,10 +215,10 @@ def _best(M: int, N: int, K: int, forms) -> tuple:
 @functools.lru_cache(4096)
 def _linear_form(M: int, N: int, K: int) -> tuple:
     """(0, rows, 16 columns) of the few-row kernel or (1, mj, ni) of the tiles for x [M, K] against a weight [N, K]."""
-    return _best(M, N, K, _ROWS + _TILES if M > 64 else [f for f in _ROWS if f[0] >= min(M, 16)])
+    return _best(M, N, K, _ROWS + _TILES)
 
 
-# both operands in 4 bits (64 x 16 results 6.2 / 11.5, 64 x 128 12 / 22, 128 x 64 11.7 / 22, 16 x 16 4.8 / 8; 256 x 128 33 / 72, 256 x 256 49 / 104)
+# both operands in 4 bits
 _MATMUL = ([(xr, 16 * rt, (0, xr, rt), (a + b * rt) / 2, f + g * rt)
             for xr, a, b, f, g, rts in ((16, 0.05, 0.0125, 2.9, 0.1, (1, 2, 4, 6, 8)), (32, 0.05, 0.015, 3.3, 0.1, (1, 2, 4, 6, 8)),
                                         (64, 0.087, 0.013, 2.8, 0.4, (1, 2, 3, 4, 6, 8)), (128, 0.0, 0.048, 0.0, 1.4, (4,)))
@@ -232,15 +232,14 @@ def _matmul_form(M: int, N: int, K: int) -> tuple:
     return _best(M, N, K, _MATMUL)
 
 
-# the gradient likewise, a stage 64 of the weight's rows (4096 / 12288 of them: 64 x 128 results 24 / 60, 32 x 128 17 / 42, 16 x 128 13 / 30; 128 x
-# 256 72 / 200; 509 x 4096 x 4096 on 64 x 128 26, on 64 x 256 tiles 48)
+# the gradient likewise, a stage 64 of the weight's rows
 _GRAD = ([(xr, 128, (0, xr, 0), c, e) for xr, c, e in ((16, 0.15, 4.5), (32, 0.21, 4.6), (64, 0.28, 5.4))]
-         + [(32 * mj, 256, (1, mj, 2), c, e) for mj, c, e in ((4, 0.83, 11.5), (8, 1.4, 13.0))])
+         + [(32 * mj, 256, (1, mj, 0), c, e) for mj, c, e in ((4, 0.83, 11.5), (8, 1.4, 13.0))])
 
 
 @functools.lru_cache(4096)
 def _grad_form(M: int, N: int, K: int) -> tuple:
-    """(0, rows, 0) of the few-row kernel or (1, mj, wn) of the tiles for dy [M, N] against a weight [N, K]."""
+    """(0, rows, 0) of the few-row kernel or (1, mj, 0) of the tiles for dy [M, N] against a weight [N, K]."""
     return _best(M, K, N, _GRAD)
 
 
