@@ -85,7 +85,7 @@ class MXFP4:
         return self.data.numel()
 
     def to(self, device) -> "MXFP4":
-        return of_data(self.data.to(device), self.shape)
+        return of_data(self.data.to(device=device), self.shape)
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         return mxfp4_dequantize(self, dtype)

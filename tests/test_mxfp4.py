@@ -144,3 +144,14 @@ def test_refusals():
     refused(mxfp4_linear, torch.zeros(1, 1 << 23), long)
     refused(mxfp4_matmul, long, long)
     refused(MXFP4, u8(1, (1 << 22) + 4), u8(1, (1 << 18) + 1))
+    with pytest.raises(TypeError):
+        w.to(torch.float16)                               # (a device: its type is the format)
+
+
+def test_matrices_pickle_and_copy():
+    import copy
+    import pickle
+
+    q = mxfp4_quantize(torch.randn(5, 72))
+    for c in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), q.to("cpu")):
+        assert c.shape == q.shape and torch.equal(c.data, q.data)

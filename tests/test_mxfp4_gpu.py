@@ -408,3 +408,94 @@ def test_a_bias_between_other_values():
         a = mxfp4_quantize(x)
         A = ref.values(a)
         ref.close(mxfp4_matmul(a, q, b), A @ W.t() + B, A.abs() @ W.abs().t() + B.abs(), 97, torch.bfloat16)
+
+
+def test_the_graph_of_a_call():
+    """What autograd promises of any node: a second pass only if kept, saved tensors through hooks and guarded against changes, no
+    forward mode."""
+    import torch.autograd.forward_ad as fwad
+
+    q, W = weight(1, 60, 96)
+    x = randn(1, 7, 96).bfloat16().requires_grad_()
+    dy = randn(2, 7, 60).bfloat16()
+    D = dy.double().cpu()
+    y = mxfp4_linear(x, q)
+    (a,) = torch.autograd.grad(y, x, dy, retain_graph=True)
+    (b,) = torch.autograd.grad(y, x, dy)
+    ref.close(a, D @ W, D.abs() @ W.abs(), 60, torch.bfloat16)
+    assert torch.equal(a, b)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, x, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = mxfp4_linear(x, q)
+    (c,) = torch.autograd.grad(y, x, dy)
+    assert torch.equal(a, c)
+    other = MXFP4(q.codes, q.scales)
+    y = mxfp4_linear(x, other)
+    other.data.zero_()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, x, dy)
+    with fwad.dual_level():
+        with pytest.raises(ValueError):
+            mxfp4_linear(fwad.make_dual(x.detach(), torch.ones_like(x)), q)
+    with torch.no_grad():
+        assert mxfp4_linear(x, q).grad_fn is None
+    z = mxfp4_linear(x.view(7, 1, 96), q).sum()          # (a gradient whose rows all lie at one address)
+    z.backward()
+    one = torch.ones(7, 60, dtype=torch.float64)
+    ref.close(x.grad, one @ W, one @ W.abs(), 60, torch.bfloat16)
+
+
+def test_a_captured_forward_and_backward():
+    q, _ = weight(1, 500, 288)
+    x = randn(1, 70, 288).bfloat16().requires_grad_()
+    dy = randn(2, 70, 500).bfloat16()
+
+    def step():
+        y = mxfp4_linear(x, q)
+        (dx,) = torch.autograd.grad(y, x, dy)
+        return y.detach(), dx
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            x.copy_(randn(10 + i, 70, 288))
+            dy.copy_(randn(20 + i, 70, 500))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_two_threads():
+    """Calls of two host threads, each on its stream."""
+    import threading
+
+    q, _ = weight(1, 1000, 512)
+    xs = [randn(i, 40 + 60 * i, 512).bfloat16() for i in range(2)]
+    want = [(mxfp4_linear(x, q), mxfp4_matmul(mxfp4_quantize(x), q)) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                y, z = mxfp4_linear(xs[i], q), mxfp4_matmul(mxfp4_quantize(xs[i]), q)
+            torch.cuda.current_stream().synchronize()
+            if not (torch.equal(y, want[i][0]) and torch.equal(z, want[i][1])):
+                bad.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
