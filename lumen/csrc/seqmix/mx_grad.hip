@@ -4,8 +4,8 @@
 // The sum runs over the weight's rows, which the codes do not lie along: a matrix instruction wants 8 rows' values of one column in a
 // lane.  A lane takes four bytes of 8 rows, makes pairs of neighbouring columns and exchanges halves between two rows (v_perm): 4
 // conversions and 4 exchanges for 8 values of two rows, where a transposed copy of the weight would cost its memory again.
-// On tiles of 128 or 256 rows x two panels: a stage (64 of the weight's rows) of 256 x 256 takes 1.40 us on all CUs, the vector unit's 16
-// units a half beside 1.25 of the forward product.  4096 rows, weight 4096 x 11008: 282 us = 1.31 PFLOP/s on 256 rows, 353 on 128;
+// On tiles of 128, 192 or 256 rows x two panels: a stage (64 of the weight's rows) of 256 x 256 takes 1.40 us on all CUs, the vector unit's 16
+// units a half beside 1.29 of the forward product.  4096 rows, weight 4096 x 11008: 282 us = 1.31 PFLOP/s on 256 rows, 353 on 128;
 // 2048 rows, 4096 x 4096: 74 on 128, 103 on 256.
 #include "mx_tile.h"
 
@@ -140,7 +140,7 @@ hipError_t sm_mx_grad(int dt, const void* dy, long long ldy, const void* codes, 
     if (dt == kBF16) grad_kernel<bf16, MJ><<<grid, 256, 0, st>>>(a);                   \
     else grad_kernel<fp16, MJ><<<grid, 256, 0, st>>>(a);                               \
     break;
-    GO(4) GO(8)
+    GO(4) GO(6) GO(8)
 #undef GO
     default: return hipErrorInvalidValue;
   }

@@ -3,9 +3,11 @@
 // The weight's values are made in x's type (exact in bf16; in fp16 rounded once: what lies below 2^-24 is lost, above 65504 infinite) and
 // multiplied by the 16-bit matrix instructions with fp32 sums, so those bound it.  A stage of 64 k of the 256 x 256 tile is, for each of
 // the four waves, 128 products of 16 cycles and between them 40 LDS reads, 64 conversions, 16 turned scales and 11 DMA pieces; alone on
-// the chip it takes 1.07 us, 0.85 being the products', on all CUs, whose clock falls with their power, 1.25.
-// A tile has 256 rows, for x is the wider operand, and 128, 192 or 256 columns, whichever fill the last round of workgroups best (us, 128 /
-// 192 / 256: 2048 x 12288 x 4096 160 / 143 / 164, 4096 x 12288 x 4096 310 / 278 / 263, 2048 x 4096 x 4096 57 / 78 / 95).
+// the chip it takes 1.07 us, 0.85 being the products', on all CUs, whose clock falls with their power, 1.25 - 1.34.
+// The larger a tile, the less its products wait (columns: 128 x 128 0.48 us a stage, 256 x 128 0.77, 256 x 256 1.29 with all CUs at work),
+// but whole rounds of 256 workgroups come and go, so there are six (us, 128 x 128 / 128 x 192 / 192 x 128 / 256 x 128 / 256 x 192 / 256 x 256: 2048 x
+// 2048 x 5632 52 / 57 / 54 / 64 / 84 / 104, 509 x 12288 x 4096 67 / 47 / 80 / 55 / 65 / 79, 1021 x 5120 x 5120 80 / 53 / 52 / 63 / 78 / 96, 4096 x 12288 x
+// 4096 - / - / - / 310 / 278 / 263).
 // 4096 x 12288 x 4096 bf16: 263 us = 1.57 PFLOP/s; the library's 16-bit product of 8192^3 runs at 1.40.
 #include "mx_tile.h"
 
@@ -61,7 +63,7 @@ hipError_t sm_mx_linear(int dt, const void* x, long long ldx, const void* codes,
     if (dt == kBF16) linear_kernel<bf16, NI, MJ, 2><<<grid, 256, 0, st>>>(a);          \
     else linear_kernel<fp16, NI, MJ, 2><<<grid, 256, 0, st>>>(a);                      \
     break;
-    GO(8, 4) GO(8, 6) GO(8, 8)
+    GO(4, 4) GO(4, 6) GO(6, 4) GO(8, 4) GO(8, 6) GO(8, 8)
 #undef GO
     default: return hipErrorInvalidValue;
   }

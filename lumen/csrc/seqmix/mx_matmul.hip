@@ -3,8 +3,9 @@
 //
 // On tiles (mx_loop.h) a stage is a panel.  256 x 256: 64 products of 16 cycles a wave between 32 LDS reads, 16 shifts and 10 DMA pieces; a
 // stage alone on the chip takes 0.61 us, 0.43 being the products' and 0.39 its 34 KB of DMA, on all CUs 0.80 (products alone, with random
-// codes: 6.4 PFLOP/s, with zeros 9.8: power).  Tiles of 256 rows x 128, 192 or 256 columns by rounds (us: 1021 x 12288 x 4096 49 / 32 / 34,
-// 4096 x 22016 x 4096 253 / 218 / 200 = 3.70 PFLOP/s).
+// codes: 6.4 PFLOP/s, with zeros 9.8: power).  Six tiles by rounds, as in mx_linear.hip (us, 256 x 128 / 256 x 192 / 256 x 256:
+// 1021 x 12288 x 4096 49 / 32 / 34, 4096 x 22016 x 4096 253 / 218 / 200 = 3.70 PFLOP/s; 128 x 128 / 128 x 192 / 256 x 128: 2048 x 2048 x 5632 22 / 26 / 31,
+// 509 x 12288 x 4096 31 / 23 / 26).
 // Few results: below.
 #include "mx_tile.h"
 
@@ -137,7 +138,7 @@ hipError_t sm_mx_matmul(int dt, const void* xc, const void* xs, const void* code
     else if (dt == kF16) matmul_kernel<fp16, NI, MJ, 2><<<grid, 256, 0, st>>>(a);      \
     else matmul_kernel<float, NI, MJ, 2><<<grid, 256, 0, st>>>(a);                     \
     break;
-    GO(8, 4) GO(8, 6) GO(8, 8)
+    GO(4, 4) GO(4, 6) GO(6, 4) GO(8, 4) GO(8, 6) GO(8, 8)
 #undef GO
     default: return hipErrorInvalidValue;
   }

@@ -198,13 +198,14 @@ def _decode(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 
 # What a round of 256 workgroups takes, us (bf16, weights from HBM), as a time a stage of 64 k and one beside them: a + b rt and f + g rt on the
-# few-row kernel's xr x 16 rt results, c and e on tiles of 32 mj x 32 ni (the kernels say what either form takes).  Over 190 sizes of 1 to
-# 4096 rows the form chosen takes 1 % more than the best one, 16 % at worst.
+# few-row kernel's xr x 16 rt results, c and e on tiles of 32 mj x 32 ni (the kernels say what either form takes).  Over 210 sizes of 1 to
+# 4096 rows the form chosen takes 0.5 % more than the best one, 15 % at worst.
 _ROWS = [(xr, 16 * rt, (0, xr, rt), a + b * rt, f + g * rt)
-         for xr, a, b, f, g, rts in ((16, 0.03, 0.0075, 1.9, 0.5, (1, 2, 3, 4, 6, 8)), (32, 0.075, 0.0135, 1.5, 0.5, (1, 2, 3, 4, 6)),
-                                     (32, 0.24, 0.0, 5.9, 0.0, (8,)), (64, 0.1, 0.02, 2.0, 0.6, (2, 3, 4, 6, 8)))
+         for xr, a, b, f, g, rts in ((16, 0.03, 0.0075, 1.8, 0.4, (1, 2, 3, 4, 6, 8)), (32, 0.065, 0.012, 1.9, 0.5, (1, 2, 3, 4, 6)),
+                                     (32, 0.21, 0.0, 5.0, 0.0, (8,)), (64, 0.09, 0.017, 2.3, 0.5, (2, 3, 4, 6, 8)))
          for rt in rts]
-_TILES = [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.75, 10.0), (6, 1.03, 11.5), (8, 1.25, 14.5))]
+_TILES = [(32 * mj, 32 * ni, (1, mj, ni), c, e)
+          for mj, ni, c, e in ((4, 4, 0.48, 9.0), (4, 6, 0.63, 7.5), (6, 4, 0.6, 8.5), (8, 4, 0.77, 8.0), (8, 6, 1.04, 9.5), (8, 8, 1.29, 12.0))]
 
 
 def _best(M: int, N: int, K: int, forms) -> tuple:
@@ -223,7 +224,8 @@ _MATMUL = ([(xr, 16 * rt, (0, xr, rt), (a + b * rt) / 2, f + g * rt)
             for xr, a, b, f, g, rts in ((16, 0.05, 0.0125, 2.9, 0.1, (1, 2, 4, 6, 8)), (32, 0.05, 0.015, 3.3, 0.1, (1, 2, 4, 6, 8)),
                                         (64, 0.087, 0.013, 2.8, 0.4, (1, 2, 3, 4, 6, 8)), (128, 0.0, 0.048, 0.0, 1.4, (4,)))
             for rt in rts]
-           + [(256, 32 * ni, (1, 8, ni), c, e) for ni, c, e in ((4, 0.27, 11.5), (6, 0.34, 12.0), (8, 0.40, 14.5))])
+           + [(32 * mj, 32 * ni, (1, mj, ni), c, e)
+              for mj, ni, c, e in ((4, 4, 0.173, 7.0), (4, 6, 0.25, 6.3), (6, 4, 0.24, 6.6), (8, 4, 0.3, 7.3), (8, 6, 0.355, 9.0), (8, 8, 0.44, 9.0))])
 
 
 @functools.lru_cache(4096)
@@ -233,8 +235,8 @@ def _matmul_form(M: int, N: int, K: int) -> tuple:
 
 
 # the gradient likewise, a stage 64 of the weight's rows
-_GRAD = ([(xr, 128, (0, xr, 0), c, e) for xr, c, e in ((16, 0.15, 4.5), (32, 0.21, 4.6), (64, 0.28, 5.4))]
-         + [(32 * mj, 256, (1, mj, 0), c, e) for mj, c, e in ((4, 0.83, 11.5), (8, 1.4, 13.0))])
+_GRAD = ([(xr, 128, (0, xr, 0), c, e) for xr, c, e in ((16, 0.15, 4.5), (32, 0.2, 4.6), (64, 0.25, 5.2))]
+         + [(32 * mj, 256, (1, mj, 0), c, e) for mj, c, e in ((4, 0.85, 11.5), (6, 1.13, 12.2), (8, 1.42, 13.3))])
 
 
 @functools.lru_cache(4096)
