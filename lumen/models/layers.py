@@ -270,7 +270,7 @@ class Linear(nn.Module):
 
     @torch.no_grad()
     def merge_lora(self):
-        """W += scale * B A for every adapted segment (serving: merge-on-load, SURVEY D16).  A quantised
+        """W += scale * B A for every adapted segment (serving: merge-on-load).  A quantised
         base is brought back to its 16-bit values first: the sum is not rounded to 4 bits."""
         lo = self.lora
         if lo is None:
