@@ -207,8 +207,9 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
   float fs[GRAD ? 2 : 1];
   const int xrow = (16 * MJ * wm + lr) * 128;
   const int wrow = 16 * NI * wn + lr;
-  // read n of half h of a stage: codes, scales (a row's four, once a stage; GRAD: the byte), fragments of x
-  constexpr int RS = RW, READS = RW + RS + MJ;
+  const int by = 9 + 8 * (lr >> 2);                      // GRAD: to the byte of the lane's columns
+  // read n of half h of a stage: codes, scales (a row's four, once a stage; GRAD: those of four rows), fragments of x
+  constexpr int RS = GRAD ? 2 : RW, READS = RW + RS + MJ;
   auto read = [&](int h, int slot, int n) __attribute__((always_inline)) {
     const char* d = lds + slot * SB;
     if (n < RW) {
@@ -220,8 +221,10 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
       }
     } else if (n < RW + RS) {
       const int u = n - RW;
-      if constexpr (GRAD) sc[u] = *reinterpret_cast<const unsigned char*>(d + XB + WB + wn * 256 + (32 * h + 8 * lg + u) * 4 + (lr >> 2));
-      else if (h == 0) sc[u] = *reinterpret_cast<const unsigned*>(d + XB + WB + (wrow + 16 * u) * 4);
+      if constexpr (GRAD) {
+        const uint4 v = *reinterpret_cast<const uint4*>(d + XB + WB + wn * 256 + (32 * h + 8 * lg + 4 * u) * 4);
+        sc[4 * u] = v.x, sc[4 * u + 1] = v.y, sc[4 * u + 2] = v.z, sc[4 * u + 3] = v.w;
+      } else if (h == 0) sc[u] = *reinterpret_cast<const unsigned*>(d + XB + WB + (wrow + 16 * u) * 4);
     } else {
       const int u = n - RW - RS;
       fx[h][u] = *reinterpret_cast<const uint4*>(d + xrow + u * 2048 + (((4 * h + lg) ^ tile::swz(16 * MJ * wm + lr)) << 4));
@@ -232,7 +235,7 @@ __device__ __forceinline__ void products(char* lds, const Walk& a, const unsigne
   auto make = [&](int h, int t, auto num) __attribute__((always_inline)) {
     constexpr int n = decltype(num)::value, w = n & 3, u = n >> 2;
     if constexpr (GRAD) {                                // rows 2 u and 2 u + 1, columns 2 w and 2 w + 1
-      if constexpr (w == 0) fs[0] = mx_scale(sc[2 * u]), fs[1] = mx_scale(sc[2 * u + 1]);
+      if constexpr (w == 0) fs[0] = mx_scale_of(sc[2 * u], by), fs[1] = mx_scale_of(sc[2 * u + 1], by);
       const uint2 v = columns<T, w>(raw[2 * u], raw[2 * u + 1], fs[0], fs[1]);
       fw[h][2 * w][u] = v.x, fw[h][2 * w + 1][u] = v.y;
     } else {
