@@ -70,8 +70,8 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_grad_kernel(const TileArgs a)
   __shared__ __attribute__((aligned(16))) char lds[NW * (S::LDS > PART ? S::LDS : PART)];
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = tile::unit_of(blockIdx.x, gridDim.x);
-  const int tm = tile % a.tiles_m, panel = tile / a.tiles_m;
+  int tm, panel;
+  tile::tile_at(tile::unit_of(blockIdx.x, gridDim.x), a.tiles_m, a.tiles_n, a.group, tm, panel);
   const int m0 = tm * XR;
   const int steps = (a.N + 63) / 64, t0 = steps * wid / NW, nk = steps * (wid + 1) / NW - t0;
   f32x4 acc[8][MT];
@@ -156,7 +156,7 @@ hipError_t sm_mx_rows_grad(int dt, const void* dy, long long ldy, const void* co
     return hipErrorInvalidValue;
   TileArgs a{dy, ldy, nullptr, codes, scales, nullptr, dx, M, N, K, Nx, 0, 0, 0, 8};
   int grid;
-  if (!mx::plan(a, K, xr, 128, grid)) return hipErrorInvalidValue;
+  if (!mx::plan(a, K, xr, 128, grid, 8)) return hipErrorInvalidValue;
   switch (xr) {
 #define GO(XR, NW)                                                                             \
   case XR:                                                                                     \

@@ -56,8 +56,8 @@ __global__ void __launch_bounds__(256, 1) rows_matmul_kernel(const TileArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[S::LDS];
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = tile::unit_of(blockIdx.x, gridDim.x);
-  const int tm = tile % a.tiles_m, tn = tile / a.tiles_m;                // the row groups of a column tile share an XCD
+  int tm, tn;                                            // (the row groups of a column tile share an XCD)
+  tile::tile_at(tile::unit_of(blockIdx.x, gridDim.x), a.tiles_m, a.tiles_n, a.group, tm, tn);
   const int m0 = tm * XR, n0 = tn * 16 * RT;
   char* ring = lds + wid * D * S::SB;
   const unsigned ring0 = __builtin_amdgcn_readfirstlane(mx::lds_addr(ring));
@@ -153,7 +153,7 @@ hipError_t sm_mx_rows_matmul(int dt, const void* xc, const void* xs, const void*
     return hipErrorInvalidValue;
   TileArgs a{xc, 0, xs, codes, scales, bias, y, M, N, K, 0, 0, 0, 0, mx::store_width(y, N, dt == kF32 ? 4 : 2)};
   int grid;
-  if (!mx::plan(a, N, xr, 16 * rt, grid)) return hipErrorInvalidValue;
+  if (!mx::plan(a, N, xr, 16 * rt, grid, 8)) return hipErrorInvalidValue;
   switch (10 * xr + rt) {
 #define GO(XR, RT, D)                                                                  \
   case 10 * XR + RT:                                                                   \

@@ -35,8 +35,8 @@ __global__ void __launch_bounds__(64 * NW, 1) rows_kernel(const TileArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[S::LDS];
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = tile::unit_of(blockIdx.x, gridDim.x);
-  const int tm = tile % a.tiles_m, tn = tile / a.tiles_m;                // the row groups of a column tile share an XCD
+  int tm, tn;                                            // (the row groups of a column tile share an XCD)
+  tile::tile_at(tile::unit_of(blockIdx.x, gridDim.x), a.tiles_m, a.tiles_n, a.group, tm, tn);
   const int m0 = tm * XR, n0 = tn * 16 * RT;
   char* ring = lds + wid * D * S::SB;
   const unsigned ring0 = __builtin_amdgcn_readfirstlane(mx::lds_addr(ring));
@@ -121,8 +121,8 @@ __global__ void __launch_bounds__(256, 1) rows_loop_kernel(const TileArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[NW * (S::LDS > PART ? S::LDS : PART)];
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = tile::unit_of(blockIdx.x, gridDim.x);
-  const int tm = tile % a.tiles_m, tn = tile / a.tiles_m;                // the row groups of a column tile share an XCD
+  int tm, tn;                                            // (the row groups of a column tile share an XCD)
+  tile::tile_at(tile::unit_of(blockIdx.x, gridDim.x), a.tiles_m, a.tiles_n, a.group, tm, tn);
   const int m0 = tm * XR, n0 = tn * 16 * RT;
   const int steps = (a.K + 63) / 64, t0 = steps * wid / NW, nk = steps * (wid + 1) / NW - t0;
   const long long wp = (long long)a.N * 64, sp = (long long)a.N * 4;
@@ -162,7 +162,7 @@ hipError_t sm_mx_rows(int dt, const void* x, long long ldx, const void* codes, c
     return hipErrorInvalidValue;
   TileArgs a{x, ldx, nullptr, codes, scales, bias, y, M, N, K, 0, 0, 0, 0, mx::store_width(y, N, 2)};
   int grid;
-  if (!mx::plan(a, N, xr, 16 * rt, grid)) return hipErrorInvalidValue;
+  if (!mx::plan(a, N, xr, 16 * rt, grid, 8)) return hipErrorInvalidValue;
   switch (10 * xr + rt) {
 #define GO(XR, RT, NW, D)                                                                \
   case 10 * XR + RT:                                                                     \

@@ -89,11 +89,12 @@ inline bool sizes_ok(int M, int N, int K) {
   return M >= 1 && N >= 1 && M <= (1 << 24) && N <= (1 << 24) && K >= 8 && K % 8 == 0 && K <= (1 << 23);
 }
 
-// grid of BM x BN tiles over M x C results; false: too many
-inline bool plan(TileArgs& a, int C, int BM, int BN, int& grid) {
+// Grid of BM x BN tiles over M x C results; false: too many.  Tiles go to an XCD by `most` groups of rows or, where there are more, by 4
+// (64 x 64 and 64 x 128 results: 1021 x 1024 x 4096 14.1 -> 12.0 us, 1021 x 4096 x 4096 38.5 -> 37.3; 5 groups by 4 rather 35.2 -> 36.3).
+inline bool plan(TileArgs& a, int C, int BM, int BN, int& grid, int most = 4) {
   const long long tm = (a.M + BM - 1LL) / BM, tn = (C + BN - 1LL) / BN;
   if (tm * tn >= (1LL << 24)) return false;
-  a.tiles_m = (int)tm, a.tiles_n = (int)tn, a.group = (int)(tm < 4 ? tm : 4);
+  a.tiles_m = (int)tm, a.tiles_n = (int)tn, a.group = (int)(tm <= most ? tm : 4);
   grid = (int)(tm * tn);
   return true;
 }
