@@ -89,16 +89,35 @@ struct Rows {
   }
 };
 
-constexpr int64_t kMaxLd = 1 << 22;
+constexpr int64_t kMaxLd = 1 << 22, kMaxRows = 1 << 24;
 typedef std::array<int, 3> Form;          // tiles or few rows, and their two sizes (lumen/ops/mxfp4.py)
 
-void need(const Tensor& x, int64_t K, const char* what) {
-  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && x.size(1) == K, what, ": no GPU rows of ", K, " values");
+void need(const Tensor& x, const char* what) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && x.size(0) <= kMaxRows, what, ": no GPU rows (at most ", kMaxRows, ")");
   TORCH_CHECK_VALUE(!x._fw_grad(0).defined(), what, ": no forward-mode derivative");
 }
 
+// 16-bit rows of K values beside the weight's data (whose size cannot tell two K of one number of panels apart); the code of their type
+int need_rows(const Tensor& x, const Tensor& data, int64_t K, const char* what) {
+  need(x, what);
+  TORCH_CHECK_VALUE(x.size(1) == K, what, ": rows of ", x.size(1), " values against a weight of ", K);
+  TORCH_CHECK_VALUE(K <= kMaxLd, what, ": rows of ", K, " values (at most ", kMaxLd, ")");
+  TORCH_CHECK_VALUE(x.device() == data.device(), what, ": rows on ", x.device(), ", weight on ", data.device());
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, what, ": rows of ", toString(x.scalar_type()),
+                    " (bf16 or fp16)");
+  return code_of(x.scalar_type(), what);
+}
+
+// a bias [N] as the kernels read it, undefined where there is none
+Tensor need_bias(const std::optional<Tensor>& bias, const Tensor& data, int64_t N, at::ScalarType type, const char* what) {
+  if (!bias) return Tensor();
+  TORCH_CHECK_VALUE(bias->device() == data.device() && bias->numel() == N && bias->scalar_type() == type, what, ": the bias is not [", N,
+                    "] values of ", toString(type), " on ", data.device());
+  return bias->contiguous();
+}
+
 Tensor quantize(const Tensor& x) {
-  need(x, x.size(-1), "mxfp4_quantize");
+  need(x, "mxfp4_quantize");
   const int dt = code_of(x.scalar_type(), "mxfp4_quantize");
   const int64_t R = x.size(0), K = x.size(1);
   Tensor data = at::empty({(K + 127) / 128 * R * 68}, x.options().dtype(at::kByte));
@@ -122,28 +141,25 @@ Tensor dequantize(const Tensor& data, int64_t R, int64_t K, at::ScalarType type)
   return y;
 }
 
-Tensor linear(const Tensor& x, const Tensor& data, int64_t N, const std::optional<Tensor>& bias, const Form& f) {
-  const int64_t M = x.size(0), K = x.size(1);
-  need(x, K, "mxfp4_linear");
-  const int dt = code_of(x.scalar_type(), "mxfp4_linear");
+Tensor linear(const Tensor& x, const Tensor& data, int64_t N, int64_t K, const std::optional<Tensor>& bias, const Form& f) {
+  const int dt = need_rows(x, data, K, "mxfp4_linear");
   const Packed w(data, N, K);
+  const Tensor b = need_bias(bias, data, N, x.scalar_type(), "mxfp4_linear");
+  const int64_t M = x.size(0);
   Tensor y = at::empty({M, N}, x.options());
   if (M && N) {
     const On on(x.device());
     const Rows r(x, 8, kMaxLd);
-    const Tensor b = bias ? bias->contiguous() : Tensor();
-    TORCH_CHECK_VALUE(!bias || (b.is_cuda() && b.numel() == N && b.scalar_type() == x.scalar_type()), "mxfp4_linear: the bias does not fit");
     done(fn<LinearFn>(f[0] ? kLinear : kRows)(dt, r.p, r.ld, w.codes, w.scales, bias ? b.data_ptr() : nullptr, y.data_ptr(), int(M), int(N),
                                               int(K), f[1], f[2], on.stream), "mxfp4_linear");
   }
   return y;
 }
 
-Tensor grad(const Tensor& dy, const Tensor& data, int64_t K, const Form& f) {
-  const int64_t M = dy.size(0), N = dy.size(1);
-  need(dy, N, "gradient of mxfp4_linear");
-  const int dt = code_of(dy.scalar_type(), "gradient of mxfp4_linear");
+Tensor grad(const Tensor& dy, const Tensor& data, int64_t N, int64_t K, const Form& f) {
+  const int dt = need_rows(dy, data, N, "gradient of mxfp4_linear");
   const Packed w(data, N, K);
+  const int64_t M = dy.size(0);
   if (!M || !N) return at::zeros({M, K}, dy.options());
   const On on(dy.device());
   Tensor dx = at::empty({M, K}, dy.options()), rows = dy;
@@ -184,7 +200,7 @@ struct Product : torch::autograd::Node {
 
 Tensor tracked(const Tensor& in, const Tensor& data, int64_t N, int64_t K, const std::optional<Tensor>& bias, const Form& f, const Form& g,
                bool back) {
-  Tensor out = back ? grad(in, data, K, g) : linear(in, data, N, bias, f);
+  Tensor out = back ? grad(in, data, N, K, g) : linear(in, data, N, K, bias, f);
   if (at::GradMode::is_enabled() && in.requires_grad()) {
     std::shared_ptr<Product> node(new Product(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(in));
@@ -195,26 +211,28 @@ Tensor tracked(const Tensor& in, const Tensor& data, int64_t N, int64_t K, const
   return out;
 }
 
-Tensor mx_linear(const Tensor& x, const Tensor& data, int64_t N, const std::optional<Tensor>& bias, int f0, int f1, int f2) {
-  return linear(x, data, N, bias, {f0, f1, f2});
+Tensor mx_linear(const Tensor& x, const Tensor& data, int64_t N, int64_t K, const std::optional<Tensor>& bias, int f0, int f1, int f2) {
+  return linear(x, data, N, K, bias, {f0, f1, f2});
 }
 
-Tensor mx_grad(const Tensor& dy, const Tensor& data, int64_t K, int g0, int g1, int g2) { return grad(dy, data, K, {g0, g1, g2}); }
+Tensor mx_grad(const Tensor& dy, const Tensor& data, int64_t N, int64_t K, int g0, int g1, int g2) {
+  return grad(dy, data, N, K, {g0, g1, g2});
+}
 
-Tensor mx_linear_tracked(const Tensor& x, const Tensor& data, int64_t N, const std::optional<Tensor>& bias, int f0, int f1, int f2, int g0,
-                         int g1, int g2) {
-  return tracked(x, data, N, x.size(1), bias, {f0, f1, f2}, {g0, g1, g2}, false);
+Tensor mx_linear_tracked(const Tensor& x, const Tensor& data, int64_t N, int64_t K, const std::optional<Tensor>& bias, int f0, int f1, int f2,
+                         int g0, int g1, int g2) {
+  return tracked(x, data, N, K, bias, {f0, f1, f2}, {g0, g1, g2}, false);
 }
 
 Tensor mx_matmul(const Tensor& x, const Tensor& data, int64_t M, int64_t N, int64_t K, const std::optional<Tensor>& bias, at::ScalarType type,
                  int f0, int f1, int f2) {
+  TORCH_CHECK_VALUE(x.device() == data.device(), "mxfp4_matmul: rows on ", x.device(), ", weight on ", data.device());
   const Packed a(x, M, K), w(data, N, K);
   const int dt = code_of(type, "mxfp4_matmul");
+  const Tensor b = need_bias(bias, data, N, type, "mxfp4_matmul");
   Tensor y = at::empty({M, N}, x.options().dtype(type));
   if (M && N) {
     const On on(x.device());
-    const Tensor b = bias ? bias->contiguous() : Tensor();
-    TORCH_CHECK_VALUE(!bias || (b.is_cuda() && b.numel() == N && b.scalar_type() == type), "mxfp4_matmul: the bias does not fit");
     done(fn<MatmulFn>(f0 ? kMatmul : kRowsMatmul)(dt, a.codes, a.scales, w.codes, w.scales, bias ? b.data_ptr() : nullptr, y.data_ptr(), int(M),
                                                   int(N), int(K), f1, f2, on.stream), "mxfp4_matmul");
   }

@@ -263,20 +263,20 @@ def _check(name: str, K: int, device, w, bias: Optional[torch.Tensor], dtype: to
 
 
 def linear_rows(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``mxfp4_linear`` of checked rows [M, K], on the GPU without autograd."""
-    (M, K), N = x.shape, w.shape[0]
+    """``mxfp4_linear`` of rows [M, K], on the GPU without autograd (and checked there by the extension alone)."""
+    M, (N, K) = x.shape[0], w.shape
     if not x.is_cuda:
         y = x.float() @ _decode(w.codes, w.scales).to(x.dtype).float().t()
         return (y if bias is None else y + bias.float()).to(x.dtype)
-    return (_calls or _native_calls()).mx_linear(x, w.data, N, bias, *_linear_form(M, N, K))
+    return (_calls or _native_calls()).mx_linear(x, w.data, N, K, bias, *_linear_form(M, N, K))
 
 
 def input_grad(dy: torch.Tensor, w: MXFP4) -> torch.Tensor:
     """dx [M, K] = dy [M, N] times the weight's values in dy's type."""
-    (M, N), K = dy.shape, w.shape[1]
+    M, (N, K) = dy.shape[0], w.shape
     if not dy.is_cuda:
         return (dy.float() @ _decode(w.codes, w.scales).to(dy.dtype).float()).to(dy.dtype)
-    return (_calls or _native_calls()).mx_grad(dy, w.data, K, *_grad_form(M, N, K))
+    return (_calls or _native_calls()).mx_grad(dy, w.data, N, K, *_grad_form(M, N, K))
 
 
 def mxfp4_linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -293,7 +293,7 @@ def mxfp4_linear(x: torch.Tensor, w: MXFP4, bias: Optional[torch.Tensor] = None)
         (M, K), N = x2.shape, w.shape[0]
         if N > MAX_LD:
             raise ValueError(f"mxfp4_linear: {N} columns with a gradient (at most {MAX_LD})")
-        y = (_calls or _native_calls()).mx_linear_tracked(x2, w.data, N, bias, *_linear_form(M, N, K), *_grad_form(M, N, K))
+        y = (_calls or _native_calls()).mx_linear_tracked(x2, w.data, N, K, bias, *_linear_form(M, N, K), *_grad_form(M, N, K))
     else:
         y = linear_rows(x2, w, bias)
     return y if len(sh) == 2 else y.view(*sh[:-1], w.shape[0])

@@ -499,3 +499,28 @@ def test_two_threads():
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("K", [256, 248])
+def test_rows_of_another_width_are_refused(K):
+    """Rows whose last panel is the weight's own last one too: their bytes alone fit."""
+    q, _ = weight(1, 40, K)
+    for other in (K - 8, K + 8, K - 128):
+        x = randn(1, 5, other).bfloat16()
+        for f in (lambda: mx.linear_rows(x, q), lambda: mxfp4_linear(x, q), lambda: mxfp4_linear(x.requires_grad_(), q)):
+            with pytest.raises(ValueError):
+                f()
+    for n in (32, 39, 41, 48):
+        with pytest.raises(ValueError):
+            mx.input_grad(randn(1, 5, n).bfloat16(), q)
+
+
+def test_rows_and_weights_the_extension_refuses():
+    """What the calls under autograd functions hand over unchecked: rows of 32 bits, a weight on the host, a bias of other size."""
+    q, _ = weight(1, 40, 256)
+    x = randn(1, 5, 256).bfloat16()
+    for f in (lambda: mx.linear_rows(x.float(), q), lambda: mx.input_grad(randn(1, 5, 40), q), lambda: mx.linear_rows(x, q.to("cpu")),
+              lambda: mx.input_grad(randn(1, 5, 40).bfloat16(), q.to("cpu")), lambda: mx.linear_rows(x, q, randn(1, 41).bfloat16()),
+              lambda: mx.linear_rows(x, q, randn(1, 40)), lambda: mx.linear_rows(x, q, torch.zeros(40, dtype=torch.bfloat16))):
+        with pytest.raises(ValueError):
+            f()

@@ -163,3 +163,19 @@ def test_engine_with_inputs_in_4_bits_too(graphs):
             with torch.no_grad():
                 with_q, without = (mod(ids).float().view(pos + 1, -1)[-1] for mod in (rows, plain))
             assert (logits[i] - with_q).norm() <= (with_q - without).norm() + 3e-2 * without.norm()
+
+
+@pytest.mark.parametrize("lora", [False, True])
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_quantised_linear_refuses_other_rows(lora, grad):
+    lin = Linear(256, 128, dtype=torch.bfloat16, device="cuda", seg_names=["q_proj"])
+    with torch.no_grad():
+        lin.weight.normal_(0, 0.05)
+        if lora:
+            lin.add_lora(["q_proj"], 16, 32.0, 0.0)
+    lin.quantize_base()
+    for K in (248, 264, 128):
+        x = torch.randn(6, K, device="cuda").bfloat16().requires_grad_(grad)
+        with pytest.raises(ValueError):
+            lin(x)
+    assert lin(torch.randn(6, 256, device="cuda").bfloat16()).shape == (6, 128)
