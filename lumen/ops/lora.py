@@ -528,7 +528,9 @@ class _LoraLinear(torch.autograd.Function):
         W = weight_fn() if fold is None else None
 
         def gemm():
-            y_ = matmul_nt(x2d, W) if type(W) is not MXFP4 else _mx_linear(x2d, W)
+            if type(W) is MXFP4:           # (the bias joins the fp32 sums)
+                return _mx_linear(x2d, W, bias)
+            y_ = matmul_nt(x2d, W)
             if bias is not None:
                 y_.add_(bias)
             return y_
@@ -601,9 +603,12 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2d, weight_fn, bias, w_param, wt_fn):
         W = weight_fn()
-        y = mm_nt(x2d, W) if type(W) is not MXFP4 else _mx_linear(x2d, W)
-        if bias is not None:
-            y.add_(bias)
+        if type(W) is MXFP4:
+            y = _mx_linear(x2d, W, bias)
+        else:
+            y = mm_nt(x2d, W)
+            if bias is not None:
+                y.add_(bias)
         ctx.weight_fn = weight_fn
         ctx.wt_fn = wt_fn
         ctx.w_grad = w_param is not None and w_param.requires_grad

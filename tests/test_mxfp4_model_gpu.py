@@ -179,3 +179,23 @@ def test_a_quantised_linear_refuses_other_rows(lora, grad):
         with pytest.raises(ValueError):
             lin(x)
     assert lin(torch.randn(6, 256, device="cuda").bfloat16()).shape == (6, 128)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("lora", [False, True])
+def test_a_bias_is_added_before_the_rounding(lora, dtype):
+    """A quantised projection with a bias gives mxfp4_linear's own bits: fp32 sums and the bias, one rounding."""
+    from lumen.ops.mxfp4 import mxfp4_linear
+
+    lin = Linear(256, 384, bias=True, dtype=dtype, device="cuda", seg_names=["fc1"])
+    g = torch.Generator(device="cuda").manual_seed(5)
+    with torch.no_grad():
+        lin.weight.normal_(0, 0.05, generator=g)
+        lin.bias.normal_(0, 1, generator=g)
+        if lora:                                          # lora_B is zero: the adapter adds nothing
+            lin.add_lora(["fc1"], 16, 32.0, 0.0)
+    lin.quantize_base()
+    for T in (1, 70, 600):
+        x = torch.randn(T, 256, device="cuda", generator=g).to(dtype)
+        same = torch.equal(lin(x), mxfp4_linear(x, lin.qweight, lin.bias))
+        assert same
