@@ -113,7 +113,7 @@ Tensor need_bias(const std::optional<Tensor>& bias, const Tensor& data, int64_t 
   if (!bias) return Tensor();
   TORCH_CHECK_VALUE(bias->device() == data.device() && bias->numel() == N && bias->scalar_type() == type, what, ": the bias is not [", N,
                     "] values of ", toString(type), " on ", data.device());
-  return bias->contiguous();
+  return bias->resolve_neg().contiguous();
 }
 
 Tensor quantize(const Tensor& x) {

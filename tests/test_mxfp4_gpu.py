@@ -524,3 +524,14 @@ def test_rows_and_weights_the_extension_refuses():
               lambda: mx.linear_rows(x, q, randn(1, 40)), lambda: mx.linear_rows(x, q, torch.zeros(40, dtype=torch.bfloat16))):
         with pytest.raises(ValueError):
             f()
+
+
+def test_a_negated_bias_of_one_value():
+    """A view whose sign torch keeps beside its memory: the imaginary part of a conjugate."""
+    q, W = weight(3, 1, 64)
+    x = randn(1, 4, 64).bfloat16()
+    a = mxfp4_quantize(x)
+    A = ref.values(a)
+    b = torch.complex(torch.zeros(1), torch.full((1,), 3.0)).cuda().conj().imag
+    assert b.is_neg() and float(b) == -3
+    ref.close(mxfp4_matmul(a, q, b, out_dtype=torch.float32), A @ W.t() - 3, A.abs() @ W.abs().t() + 3, 65, torch.float32)
