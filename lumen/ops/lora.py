@@ -658,8 +658,12 @@ def linear(x: torch.Tensor, weight_fn, bias: Optional[torch.Tensor] = None,
 
 
 def _base(x2d, W, bias):
-    """The torch path of the base product, W in x's type or in MXFP4."""
-    return F.linear(x2d, W, bias) if type(W) is not MXFP4 else mxfp4_linear(x2d, W, bias)
+    """The torch path of the base product, W in x's type or in MXFP4 (whose product has no gradient of a bias)."""
+    if type(W) is not MXFP4:
+        return F.linear(x2d, W, bias)
+    if bias is not None and bias.requires_grad:
+        return mxfp4_linear(x2d, W) + bias
+    return mxfp4_linear(x2d, W, bias)
 
 
 def _frozen(W):

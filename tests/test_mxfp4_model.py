@@ -223,3 +223,22 @@ def test_hybrid_models_and_zero3_refuse(tmp_path):
         ZeroEngine(m, ds, env)
     with pytest.raises(ValueError, match="ZeRO-3"):
         Trainer(TrainArgs(model_name="tiny-llama", init="random", synthetic=True, base_quantization="mxfp4"), ds, env)
+
+
+@pytest.mark.parametrize("lora", [False, True])
+def test_a_bias_that_trains(lora):
+    """Its gradient is the column sums of dy, with and without adapters."""
+    lin = Linear(64, 24, bias=True, dtype=torch.float32, seg_names=["fc1"])
+    torch.manual_seed(0)
+    with torch.no_grad():
+        lin.weight.normal_(0, 0.05), lin.bias.normal_()
+        if lora:
+            lin.add_lora(["fc1"], 4, 8.0, 0.0)
+    frozen = copy.deepcopy(lin)
+    lin.bias.requires_grad_(True)
+    lin.quantize_base(), frozen.quantize_base()
+    x, dy = torch.randn(5, 64), torch.randn(5, 24)
+    y = lin(x)
+    y.backward(dy)
+    close(y.detach(), frozen(x).detach())
+    close(lin.bias.grad, dy.sum(0))
