@@ -95,6 +95,9 @@ def count_parameters(model: nn.Module):
     total = 0
     for p in model.parameters():
         total += int(torch.Size(getattr(p, "_zero_shape", p.shape)).numel())
+    # a weight in 4 bits is a buffer beside an empty parameter
+    total += sum(m.in_features * m.out_features for m in model.modules()
+                 if isinstance(m, Linear) and m.qdata is not None)
     return trainable, total
 
 

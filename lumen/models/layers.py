@@ -102,7 +102,6 @@ class Linear(nn.Module):
             raise ValueError("quantize_base: the weight is partitioned (ZeRO-3): quantise at stages 0 - 2")
         self.qdata = mxfp4_quantize(W).data
         self.weight = nn.Parameter(W.new_empty(0), requires_grad=False)
-        self.weight._zero_shape = W.shape  # (parameter counts go by it)
         self.invalidate_weight_cache()
 
     @torch.no_grad()

@@ -242,3 +242,23 @@ def test_a_bias_that_trains(lora):
     y.backward(dy)
     close(y.detach(), frozen(x).detach())
     close(lin.bias.grad, dy.sum(0))
+
+
+def test_counts_of_copies():
+    """Copied, pickled and reloaded models count a 4-bit weight as the weight that it is."""
+    import io
+    import pickle
+
+    m, plain = pair()
+    want = count_parameters(plain)
+    buf = io.BytesIO()
+    torch.save(m.state_dict(), buf)
+    buf.seek(0)
+    again = copy.deepcopy(m)
+    again.load_state_dict(torch.load(buf, weights_only=True), assign=True)
+    assert count_parameters(m) == want
+    for c in (copy.deepcopy(m), pickle.loads(pickle.dumps(m)), m.to(torch.bfloat16)):
+        assert count_parameters(c) == want
+    assert count_parameters(again)[1] == want[1]          # (what trains is not part of the state)
+    m.layers[0].mlp.down_proj.dequantize_base()
+    assert count_parameters(m) == want
