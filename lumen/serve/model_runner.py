@@ -116,8 +116,8 @@ class ServeWeights:
     def __init__(self, model, tp_rank: int = 0, tp_size: int = 1, quantization: Optional[str] = None,
                  release: bool = False):
         """``quantization`` "mxfp4": the projections of this rank's slice in 4 bits (``ops/mxfp4.py``), the LM head and the
-        embeddings as they are; "mxfp4_a4": their inputs too, quantised row by row as they come.  ``release``: the model is the caller's to spend, a layer's 16-bit projections are freed as
-        their quantised form is made."""
+        embeddings as they are; "mxfp4_a4": their inputs too, quantised row by row as they come.  ``release``: the model is the
+        caller's to spend, a layer's 16-bit projections are freed as their quantised form is made."""
         if quantization not in QUANTIZATIONS:
             raise ValueError(f"quantization must be one of {QUANTIZATIONS}, got {quantization!r}")
         self.quantization = quantization
@@ -135,27 +135,36 @@ class ServeWeights:
         qs, ks = nh * D, nkv * D
         lq, lk, lf = self.nh * D, self.nkv * D, self.F
         self.layers: List[LayerW] = []
+
+        def projections(L):
+            W = _values(L.self_attn.qkv_proj)
+            qkv = torch.cat([W[r * lq:(r + 1) * lq], W[qs + r * lk:qs + (r + 1) * lk],
+                             W[qs + ks + r * lk:qs + ks + (r + 1) * lk]], 0).contiguous()
+            o = _values(L.self_attn.o_proj)[:, r * lq:(r + 1) * lq].contiguous()
+            GU = _values(L.mlp.gate_up_proj)
+            gu = torch.cat([GU[r * lf:(r + 1) * lf], GU[Fd + r * lf:Fd + (r + 1) * lf]],
+                           0).contiguous()
+            dn = _values(L.mlp.down_proj)[:, r * lf:(r + 1) * lf].contiguous()
+            if quantization is None:
+                return qkv, o, gu, dn
+            for n, w in (("o", o), ("down", dn), ("q|k|v", qkv)):
+                if w.shape[1] % 8:
+                    raise ValueError(f"quantization: {n} has {w.shape[1]} inputs a rank, no multiple of 8")
+            return tuple(mxfp4_quantize(w) for w in (qkv, o, gu, dn))
+
+        # What a layer's 16-bit weights leave goes back to the device before the next one is quantised: a 4-bit matrix in a
+        # corner of a freed block would hold all of it, which neither the cache's sizing nor its large tensors could use.
+        on_gpu = quantization is not None and model.embed_tokens.weight.is_cuda
         with torch.no_grad():
             for L in model.layers:
-                W = _values(L.self_attn.qkv_proj)
-                qkv = torch.cat([W[r * lq:(r + 1) * lq], W[qs + r * lk:qs + (r + 1) * lk],
-                                 W[qs + ks + r * lk:qs + ks + (r + 1) * lk]], 0).contiguous()
-                o = _values(L.self_attn.o_proj)[:, r * lq:(r + 1) * lq].contiguous()
-                GU = _values(L.mlp.gate_up_proj)
-                gu = torch.cat([GU[r * lf:(r + 1) * lf], GU[Fd + r * lf:Fd + (r + 1) * lf]],
-                               0).contiguous()
-                dn = _values(L.mlp.down_proj)[:, r * lf:(r + 1) * lf].contiguous()
-                if quantization is not None:
-                    for n, w in (("o", o), ("down", dn), ("q|k|v", qkv)):
-                        if w.shape[1] % 8:
-                            raise ValueError(f"quantization: {n} has {w.shape[1]} inputs a rank, no multiple of 8")
-                    qkv, o, gu, dn = (mxfp4_quantize(w) for w in (qkv, o, gu, dn))
-                    if release:
-                        del W, GU
-                        for lin in (L.self_attn.qkv_proj, L.self_attn.o_proj, L.mlp.gate_up_proj, L.mlp.down_proj):
-                            lin.weight = torch.nn.Parameter(lin.weight.new_empty(0), requires_grad=False)
-                self.layers.append(LayerW(L.input_layernorm.weight, L.post_attention_layernorm.weight,
-                                          qkv, o, gu, dn))
+                if on_gpu:
+                    torch.cuda.empty_cache()
+                self.layers.append(LayerW(L.input_layernorm.weight, L.post_attention_layernorm.weight, *projections(L)))
+                if quantization is not None and release:
+                    for lin in (L.self_attn.qkv_proj, L.self_attn.o_proj, L.mlp.gate_up_proj, L.mlp.down_proj):
+                        lin.weight = torch.nn.Parameter(lin.weight.new_empty(0), requires_grad=False)
+            if on_gpu:
+                torch.cuda.empty_cache()
         self.embed = model.embed_tokens.weight
         self.norm = model.norm.weight
         # vocab-parallel LM head: each rank scores V/TP rows, logits all-gathered

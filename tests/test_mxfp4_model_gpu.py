@@ -199,3 +199,35 @@ def test_a_bias_is_added_before_the_rounding(lora, dtype):
         x = torch.randn(T, 256, device="cuda", generator=g).to(dtype)
         same = torch.equal(lin(x), mxfp4_linear(x, lin.qweight, lin.bias))
         assert same
+
+
+def test_memory_of_the_16_bit_projections_is_given_back():
+    """Freed projections are the device's again, so that the automatic number of cache blocks goes by what is left."""
+    import gc
+
+    from lumen.serve.engine import EngineConfig, LLMEngine
+    from lumen.serve.model_runner import ServeWeights
+
+    gc.collect()                                          # (what earlier tests left)
+    name = "llama2-70b-2l"                                # 3.4 GB of projections
+    m = build_model(name, dtype=torch.bfloat16, device="cuda", init="random")
+    held = sum(p.numel() * 2 for n, p in m.named_parameters() if "_proj" in n)
+    torch.cuda.empty_cache()
+    before = torch.cuda.mem_get_info()[0]
+    w = ServeWeights(m, quantization="mxfp4", release=True)
+    kept = sum(q.nbytes for L in w.layers for q in (L.qkv, L.o, L.gate_up, L.down))
+    assert torch.cuda.mem_get_info()[0] - before >= held - kept - (128 << 20)     # (segments are rounded up)
+    del m, w
+    gc.collect()
+    torch.cuda.empty_cache()
+    total = torch.cuda.mem_get_info()[1]
+    blocks = {}
+    for how in (None, "mxfp4"):
+        eng = LLMEngine(EngineConfig(model=name, device="cuda", max_model_len=4096, max_num_seqs=256, block_size=16, init="random",
+                                     use_graphs=False, quantization=how, gpu_memory_utilization=(14 << 30) / total))
+        blocks[how] = eng.blocks.num_blocks
+        del eng
+        gc.collect()
+        torch.cuda.empty_cache()
+    per_block = 16 * 2 * 2 * 8 * 128 * 2                  # tokens, keys and values, layers, heads, values, bytes
+    assert (blocks["mxfp4"] - blocks[None]) * per_block >= held - kept - (128 << 20)
