@@ -37,7 +37,7 @@ from ..ops.attention import (flash_attention_fresh, flash_attention_paged, paged
                              rope_write_kv)
 from ..ops.gemm import decoded_rows, linear_nt, row_norm_linear, row_norm_ok, swiglu_linear_nt
 from ..ops.moe import MID_MAX_M, THIN_ACT_MAX_M, mid_act, mid_act_ok, thin_act, thin_act_ok, tile_act, tile_act_ok
-from ..ops.mxfp4 import mxfp4_linear, mxfp4_matmul, mxfp4_quantize
+from ..ops.mxfp4 import BLOCK, mxfp4_linear, mxfp4_matmul, mxfp4_quantize
 from ..ops.norm import rms_norm
 from ..ops.rope import rope_tables
 
@@ -150,6 +150,10 @@ class ServeWeights:
             for n, w in (("o", o), ("down", dn), ("q|k|v", qkv)):
                 if w.shape[1] % 8:
                     raise ValueError(f"quantization: {n} has {w.shape[1]} inputs a rank, no multiple of 8")
+            # blocks that a cut leaves in parts of two would be rounded a second time: 4-bit values stay what they are
+            for n, lin, k in (("o", L.self_attn.o_proj, lq), ("down", L.mlp.down_proj, lf)):
+                if lin.qdata is not None and tp_size > 1 and k % BLOCK:
+                    raise ValueError(f"quantization: {n} is in 4 bits already and would be cut inside a block ({k} inputs a rank)")
             return tuple(mxfp4_quantize(w) for w in (qkv, o, gu, dn))
 
         # What a layer's 16-bit weights leave goes back to the device before the next one is quantised: a 4-bit matrix in a

@@ -262,3 +262,22 @@ def test_counts_of_copies():
     assert count_parameters(again)[1] == want[1]          # (what trains is not part of the state)
     m.layers[0].mlp.down_proj.dequantize_base()
     assert count_parameters(m) == want
+
+
+@pytest.mark.parametrize("name,cut", [("tiny-llama-tp8", False), ("tiny-llama-gqa", True)])
+def test_ranks_keep_the_values_of_a_4_bit_base(name, cut):
+    """Every rank's slice holds the base's own values; a base whose blocks the ranks would share is refused (688 / 2 is no multiple
+    of 32), and served from its 16-bit values."""
+    from lumen.serve.model_runner import ServeWeights
+
+    m, plain = pair(name, lora=False)
+    for rank in range(2):
+        if cut:
+            with pytest.raises(ValueError, match="inside a block"):
+                ServeWeights(m, rank, 2, "mxfp4")
+        whole = ServeWeights(plain, rank, 2)
+        got = ServeWeights(m, rank, 2, None if cut else "mxfp4")
+        for a, b in zip(got.layers, whole.layers):
+            for n in ("qkv", "o", "gate_up", "down"):
+                w = getattr(a, n)
+                assert torch.equal(w if cut else w.dequantize(torch.float32), getattr(b, n))
