@@ -52,7 +52,8 @@ def train_worker(rank, world, port, stage, outdir, model="tiny-llama", micro=2, 
                       "resume", False), save_final=False,
                   output_dir=ex.get("ckdir") or os.path.join(outdir, "ck"),
                   seed=7, gradient_checkpointing=(extra or {}).get("gc", False),
-                  fuse_accumulation=ex.get("fuse", True), synthetic_min_len=ex.get("min_len"))
+                  fuse_accumulation=ex.get("fuse", True), synthetic_min_len=ex.get("min_len"),
+                  base_quantization=ex.get("base_quantization"))
     try:
         t = Trainer(a, ds, env, printer=lambda *x, **k: None)
         res = t.train()
