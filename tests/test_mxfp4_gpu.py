@@ -1,5 +1,7 @@
 """The MXFP4 kernels against float64 at the edges of their tiles: every pattern of the 16-bit types, rows and columns that end
 inside a tile, k that ends inside a stage, strided rows, non-finite rows, graphs and streams."""
+import math
+
 import pytest
 import torch
 
@@ -535,3 +537,71 @@ def test_a_negated_bias_of_one_value():
     b = torch.complex(torch.zeros(1), torch.full((1,), 3.0)).cuda().conj().imag
     assert b.is_neg() and float(b) == -3
     ref.close(mxfp4_matmul(a, q, b, out_dtype=torch.float32), A @ W.t() - 3, A.abs() @ W.abs().t() + 3, 65, torch.float32)
+
+
+def test_two_threads_every_result():
+    """As above, each of 50 results compared, and a thread that raises is seen."""
+    import threading
+
+    q, _ = weight(1, 1000, 512)
+    xs = [randn(i, 40 + 60 * i, 512).bfloat16() for i in range(2)]
+    want = [(mxfp4_linear(x, q), mxfp4_matmul(mxfp4_quantize(x), q)) for x in xs]
+    torch.cuda.synchronize()
+    equal = [None, None]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [(mxfp4_linear(xs[i], q), mxfp4_matmul(mxfp4_quantize(xs[i]), q)) for _ in range(50)]
+            torch.cuda.current_stream().synchronize()
+            equal[i] = [torch.equal(a, b) for pair in got for a, b in zip(pair, want[i])]
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(e is not None and len(e) == 100 and all(e) for e in equal)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, *HALF])
+def test_blocks_of_the_smallest_numbers(dtype):
+    """Blocks whose largest value is denormal or nearly so: codes and scales as for any other."""
+    fi = torch.finfo(dtype)
+    x = randn(4, 40, 64)
+    x = (x / x.abs().amax(1, keepdim=True)).double().cpu()
+    top = torch.pow(2.0, torch.linspace(math.log2(fi.smallest_normal) - 12, math.log2(fi.smallest_normal) + 5, 40, dtype=torch.float64))
+    x = (x * top.unsqueeze(1)).to(dtype)
+    q = mxfp4_quantize(x.cuda())
+    code, byte = ref.encode(x)
+    assert torch.equal(ref.unpack(q)[1], byte) and torch.equal(ref.unpack(q)[0], code)
+
+
+@pytest.mark.parametrize("M", [3, 64, 300])
+def test_products_with_the_smallest_weights(M):
+    """Weights of 2^-128 to 2^-118, below bf16's normal numbers in part, against rows of 2^100; both in 4 bits with the smallest scales on
+    one side and the largest on the other."""
+    g = torch.Generator().manual_seed(M)
+    N, K = 80, 256
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+    q = MXFP4(codes.cuda(), torch.randint(0, 8, (N, K // 32), generator=g, dtype=torch.uint8).cuda())
+    W = ref.values(q)
+    x = (randn(1, M, K) * 2.0 ** 100).bfloat16()
+    X = x.double().cpu()
+    ref.close(mxfp4_linear(x, q), X @ W.t(), X.abs() @ W.abs().t(), K, torch.bfloat16)
+    dy = (randn(2, M, N) * 2.0 ** 100).bfloat16()
+    D = dy.double().cpu()
+    ref.close(mx.input_grad(dy, q), D @ W, D.abs() @ W.abs(), N, torch.bfloat16)
+    a = MXFP4(torch.randint(0, 256, (M, K // 2), generator=g, dtype=torch.uint8).cuda(),
+              torch.randint(235, 247, (M, K // 32), generator=g, dtype=torch.uint8).cuda())
+    A = ref.values(a)
+    ref.close(mxfp4_matmul(a, q, out_dtype=torch.float32), A @ W.t(), A.abs() @ W.abs().t(), K, torch.float32)
+
+
+@pytest.mark.parametrize("M", [3, 64, 300])
+@pytest.mark.parametrize("K", [128, 256])
+def test_zeros_under_the_largest_scales(M, K):
+    """Codes of zero times any finite scales are zero, also where the two scales' product has no fp32."""
+    q, W = weight(1, 300, K)
+    q = MXFP4(q.codes, torch.full_like(q.scales, 254))
+    a = MXFP4(torch.zeros(M, K // 2, dtype=torch.uint8).cuda(), torch.full((M, K // 32), 254, dtype=torch.uint8).cuda())
+    assert int(mxfp4_matmul(a, q, out_dtype=torch.float32).abs().max()) == 0

@@ -231,3 +231,43 @@ def test_memory_of_the_16_bit_projections_is_given_back():
         torch.cuda.empty_cache()
     per_block = 16 * 2 * 2 * 8 * 128 * 2                  # tokens, keys and values, layers, heads, values, bytes
     assert (blocks["mxfp4"] - blocks[None]) * per_block >= held - kept - (128 << 20)
+
+
+def test_engine_quantises_its_inputs_or_leaves_them():
+    """Prompts' last logits of ``mxfp4_a4`` lie nearer to the full forward on quantised rows than to the one on 16-bit rows, those of
+    ``mxfp4`` the other way round.  (Both are off by roundings that know nothing of the distance d between the two: |e|^2 of one beside
+    |e|^2 + |d|^2 of the other.)"""
+    from lumen.ops.mxfp4 import mxfp4_quantize
+    from lumen.serve.engine import EngineConfig, LLMEngine
+    from lumen.serve.sequence import SamplingParams
+
+    m, plain = pair("tiny-llama-gqa", torch.bfloat16, lora=False)
+    m.eval(), plain.eval()
+    rows = copy.deepcopy(plain)
+    for n, lin in rows.named_modules():
+        if isinstance(lin, Linear) and not n.endswith("lm_head"):
+            lin.register_forward_pre_hook(
+                lambda mod, a: (mxfp4_quantize(a[0].reshape(-1, a[0].shape[-1])).dequantize(a[0].dtype).view(a[0].shape),))
+    prompts = [list(range(10, 40)), [7, 8, 9] * 20, [42], list(range(100, 400, 3))]
+    for how, graphs in (("mxfp4", False), ("mxfp4", True), ("mxfp4_a4", False), ("mxfp4_a4", True)):
+        eng = LLMEngine(EngineConfig(model="tiny-llama-gqa", device="cuda", max_model_len=256, block_size=16, num_blocks=128,
+                                     use_graphs=graphs, quantization=how), model=m)
+        seqs = [eng.add_request(p, SamplingParams(max_tokens=6, temperature=0, ignore_eos=True)) for p in prompts]
+        got, orig = [], eng.runner.decode
+
+        def spy(inp):
+            out = orig(inp)
+            got.append((inp.positions.cpu().tolist(), out.float().clone()))
+            return out
+        eng.runner.decode = spy
+        while eng.has_work:
+            eng.step()
+        assert got
+        quantised = left = 0.0
+        for positions, logits in got:
+            for i, (s, pos) in enumerate(zip(seqs, positions)):
+                ids = torch.tensor([s.all_ids[:pos + 1]], device="cuda")
+                with torch.no_grad():
+                    quantised += float((logits[i] - rows(ids).float().view(pos + 1, -1)[-1]).norm() ** 2)
+                    left += float((logits[i] - plain(ids).float().view(pos + 1, -1)[-1]).norm() ** 2)
+        assert (quantised < left) == (how == "mxfp4_a4")
