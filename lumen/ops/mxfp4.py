@@ -141,7 +141,8 @@ def _native_calls():
 
 # ---- the format -------------------------------------------------------------------------------------
 def mxfp4_quantize(x: torch.Tensor) -> MXFP4:
-    """The MXFP4 form of x [rows, K] (fp32, bf16 or fp16; K a multiple of 8)."""
+    """The MXFP4 form of x [rows, K] (fp32, bf16 or fp16; K a multiple of 8).  No gradient passes: the result stands outside the
+    graph as that of ``x.detach()`` does, and so does what is multiplied with it (``mxfp4_linear`` has the gradient of 16-bit rows)."""
     if x.dim() != 2 or x.dtype not in DT:
         raise ValueError("mxfp4_quantize: a matrix [rows, K] of fp32, bf16 or fp16")
     R, K = x.shape

@@ -155,3 +155,13 @@ def test_matrices_pickle_and_copy():
     q = mxfp4_quantize(torch.randn(5, 72))
     for c in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), q.to("cpu")):
         assert c.shape == q.shape and torch.equal(c.data, q.data)
+
+
+def test_quantising_leaves_the_graph():
+    """Rows that want a gradient quantise as their values do, and what comes of them wants none."""
+    x = torch.randn(3, 64, requires_grad=True)
+    w = mxfp4_quantize(torch.randn(4, 64))
+    q = mxfp4_quantize(x)
+    assert torch.equal(q.data, mxfp4_quantize(x.detach()).data)
+    assert not q.dequantize(torch.float32).requires_grad and not mxfp4_matmul(q, w).requires_grad
+    assert mxfp4_linear(x, w).requires_grad
