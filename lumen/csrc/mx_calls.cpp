@@ -5,6 +5,7 @@
 // it and its gradient 90.  The launchers are in another library (lumen/_C_seqmix.so), whose loader hands their addresses over once.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <c10/core/DeviceGuard.h>
@@ -184,6 +185,7 @@ struct Product : torch::autograd::Node {
   bool back = false;                       // this node's own forward was dx = dy w
   variable_list apply(variable_list&& in) override {
     if (!in[0].defined()) return {Tensor()};
+    refuse_foreign_accumulation(in[0].device());
     Tensor d;
     {
       const std::lock_guard<std::mutex> lock(mutex_);
@@ -194,6 +196,20 @@ struct Product : torch::autograd::Node {
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
     data.reset_data();
+  }
+  // A leaf's accumulation node belongs to the stream of the first of its graphs that are alive.  If that stream is not the captured one,
+  // the engine makes it wait for the capture, which no capture survives (and an error there ends the process).
+  void refuse_foreign_accumulation(const c10::Device& device) const {
+    const auto ours = c10::hip::getCurrentHIPStream(device.index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    done(hipStreamIsCapturing(ours.stream(), &status), "gradient of mxfp4_linear");
+    if (status == hipStreamCaptureStatusNone) return;
+    auto* node = next_edge(0).function.get();
+    while (node && node->num_outputs() == 1) node = node->next_edge(0).function.get();       // (views of the leaf)
+    auto* sum = dynamic_cast<torch::autograd::AccumulateGrad*>(node);
+    const auto theirs = sum ? sum->stream() : std::nullopt;
+    TORCH_CHECK_VALUE(!theirs || theirs->id() == ours.id(), "gradient of mxfp4_linear: the captured pass ends at a leaf whose graph from "
+                      "before the capture is alive; drop that graph first");
   }
   std::string name() const override { return "Mxfp4LinearBackward"; }
 };

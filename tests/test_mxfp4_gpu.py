@@ -605,3 +605,33 @@ def test_zeros_under_the_largest_scales(M, K):
     q = MXFP4(q.codes, torch.full_like(q.scales, 254))
     a = MXFP4(torch.zeros(M, K // 2, dtype=torch.uint8).cuda(), torch.full((M, K // 32), 254, dtype=torch.uint8).cuda())
     assert int(mxfp4_matmul(a, q, out_dtype=torch.float32).abs().max()) == 0
+
+
+@pytest.mark.parametrize("shape", [(70, 288), (2, 35, 288)])
+def test_a_captured_backward_at_a_leaf_of_a_live_graph(shape):
+    """The leaf's accumulation belongs to the eager stream while a graph from before the capture is alive: refused, and possible as
+    soon as that graph is gone."""
+    q, _ = weight(1, 500, 288)
+    x = randn(1, *shape).bfloat16().requires_grad_()
+    dy = randn(2, *shape[:-1], 500).bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        (want,) = torch.autograd.grad(mxfp4_linear(x, q), x, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    live = mxfp4_linear(x, q)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="drop that graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(mxfp4_linear(x, q), x, dy)
+    (dx,) = torch.autograd.grad(live, x, dy)
+    assert torch.equal(dx, want)
+    del live
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(mxfp4_linear(x, q), x, dy)
+    for _ in range(3):
+        got.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
