@@ -5,8 +5,8 @@
 // lane.  A lane takes four bytes of 8 rows, makes pairs of neighbouring columns and exchanges halves between two rows (v_perm): 4
 // conversions and 4 exchanges for 8 values of two rows, where a transposed copy of the weight would cost its memory again.
 // On tiles of 128, 192 or 256 rows x two panels: a stage (64 of the weight's rows) of 256 x 256 takes 1.40 us on all CUs, the vector unit's 16
-// units a half beside 1.29 of the forward product.  4096 rows, weight 4096 x 11008: 275 us = 1.34 PFLOP/s on 256 rows, 296 on 192, 347 on 128;
-// 2048 rows, 4096 x 4096: 61 on 128, 103 on 256.
+// units a half beside 1.29 of the forward product.  4096 rows, weight 4096 x 11008: 282 us = 1.31 PFLOP/s on 256 rows, 305 on 192, 351 on 128;
+// 2048 rows, 4096 x 4096: 63 on 128, 90 on 256.
 #include "mx_tile.h"
 
 using namespace lumen;
@@ -61,8 +61,9 @@ __global__ void __launch_bounds__(256, 1) grad_kernel(const TileArgs a) {
 }
 
 // Few results: a workgroup takes 16 MT rows of dy and one panel of columns, its NW waves split the sum over w's rows, each in a ring of its
-// own.  16 rows leave a SIMD room for two waves.  Us: 17 rows, 4096 x 4096 11.4 on 16 (15.5 on 32), 200 rows 16.2 on 32 (20.2 on 64), 509 rows
-// 20.7 on 64 (30.5 on 32, on tiles of 128 x 256 58) = 0.83 PFLOP/s.
+// own.  16 rows leave a SIMD room for two waves.  Us: 17 rows, 4096 x 4096 11.6 on 16 (14.7 on 32), 200 rows 16.1 on 32 (19.7 on 64), 509 rows
+// 21.6 on 64 (29.3 on 32, on tiles of 128 x 256 57) = 0.79 PFLOP/s.  The sum is not split among workgroups, so few rows leave CUs idle: 17
+// rows x 4096 columns are 64 workgroups, and up to some 300 rows a call takes 3 - 6 times what its bytes do.
 template <typename T, int MT, int NW>
 __global__ void __launch_bounds__(64 * NW, 1) rows_grad_kernel(const TileArgs a) {
   using S = mx::Shape<8, MT, -NW, true>;

@@ -6,9 +6,9 @@
 // the chip it takes 1.07 us, 0.85 being the products', on all CUs, whose clock falls with their power, 1.25 - 1.34.
 // The larger a tile, the less its products wait (columns: 128 x 128 0.48 us a stage, 256 x 128 0.77, 256 x 256 1.29 with all CUs at work),
 // but whole rounds of 256 workgroups come and go, so there are six (us, 128 x 128 / 128 x 192 / 192 x 128 / 256 x 128 / 256 x 192 / 256 x 256: 2048 x
-// 2048 x 5632 52 / 57 / 54 / 64 / 84 / 104, 509 x 12288 x 4096 67 / 47 / 80 / 55 / 65 / 79, 1021 x 5120 x 5120 80 / 53 / 52 / 63 / 78 / 96, 4096 x 12288 x
-// 4096 - / - / - / 310 / 278 / 263).
-// 4096 x 12288 x 4096 bf16: 263 us = 1.57 PFLOP/s; the library's 16-bit product of 8192^3 runs at 1.40.
+// 2048 x 5632 46 / 57 / 54 / 64 / 84 / 104, 509 x 12288 x 4096 66 / 50 / 80 / 50 / 64 / 79, 1021 x 5120 x 5120 79 / 53 / 55 / 59 / 77 / 96, 4096 x 12288 x
+// 4096 - / - / - / 320 / 290 / 269).
+// 4096 x 12288 x 4096 bf16: 269 us = 1.53 PFLOP/s; the library's 16-bit product of 8192^3 runs at 1.36 on the same card.
 #include "mx_tile.h"
 
 using namespace lumen;

@@ -4,7 +4,7 @@
 // On tiles (mx_loop.h) a stage is a panel.  256 x 256: 64 products of 16 cycles a wave between 32 LDS reads, 16 shifts and 10 DMA pieces; a
 // stage alone on the chip takes 0.61 us, 0.43 being the products' and 0.39 its 34 KB of DMA, on all CUs 0.80 (products alone, with random
 // codes: 6.4 PFLOP/s, with zeros 9.8: power).  Six tiles by rounds, as in mx_linear.hip (us, 256 x 128 / 256 x 192 / 256 x 256:
-// 1021 x 12288 x 4096 49 / 32 / 34, 4096 x 22016 x 4096 253 / 218 / 200 = 3.70 PFLOP/s; 128 x 128 / 128 x 192 / 256 x 128: 2048 x 2048 x 5632 22 / 26 / 31,
+// 1021 x 12288 x 4096 48 / 32 / 33, 4096 x 22016 x 4096 268 / 229 / 210 = 3.52 PFLOP/s; 128 x 128 / 128 x 192 / 256 x 128: 2048 x 2048 x 5632 22 / 26 / 31,
 // 509 x 12288 x 4096 31 / 23 / 26).
 // Few results: below.
 #include "mx_tile.h"
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(256, 1) matmul_kernel(const TileArgs a) {
 // Few results: a workgroup takes XR rows and 16 RT columns, its four waves split k, each in a ring of its own (seqmix/mx_rows.hip); a
 // stage is a panel.  Bound by bytes: a CU takes 97 B/ns from L2, and 64 x 128 results are 13 KB a panel for 32 products.  The interleaved
 // loop of the tiles brings nothing here (64 x 22016 x 4096 13.9 -> 14.6 us, 1021 x 2048 x 5632 12.6 -> 12.7).  1 x 4096 x 4096 4.4 us, 48 x
-// 12288 x 4096 9.4 = 2.8 TB/s of weight; against tiles 509 x 4096 x 4096 11 (256 x 128: 25), 1021 x 2048 x 5632 12.6 (32).
+// 12288 x 4096 9.4 = 2.8 TB/s of weight; against tiles 509 x 4096 x 4096 11 (256 x 128: 23), 1021 x 2048 x 5632 12.9 (30).
 template <int XR, int RT, int D>
 struct Ring {
   static constexpr int NW = 4, MT = XR / 16, XB = MT * 1024, WB = RT * 1024, SX = (MT + 3) / 4, SW = (RT + 3) / 4;

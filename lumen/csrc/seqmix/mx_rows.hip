@@ -4,13 +4,15 @@
 // in LDS, filled by LDS-DMA.  No barrier stands in the loop: a wave waits for its own stages by a counted vmcnt.  The waves' sums
 // meet in LDS at the end, in wave order.  The weight's codes become 16-bit fragments in registers, by the scaled conversions.
 //  * Up to 32 rows it is bound by the weight's bytes and by the launch: stages of 128 k, whole lines of the weight, reads in a row
-//    before the products (us: 1 x 4096 x 4096 4.8, 8 x 22016 x 4096 11.9 = 4.0 TB/s of weight, 17 x 32000 x 2048 12.9).
+//    before the products (us: 1 x 4096 x 4096 4.9, 8 x 22016 x 4096 12.0 = 4.0 TB/s of weight, 17 x 32000 x 2048 12.8).
 //  * 64 rows, and 32 with 128 columns, are bound by the matrix core, the DMA and what a wave issues in turn: the tiles' loop, where each
-//    stands between products, 64 k a stage (509 x 4096 x 4096 23.9 -> 19.9 us = 0.86 PFLOP/s, 64 x 22016 x 4096 22.2 -> 20.2; 32 x 12288 x
+//    stands between products, 64 k a stage (509 x 4096 x 4096 23.9 -> 20.4 us = 0.84 PFLOP/s, 64 x 22016 x 4096 22.2 -> 20.1; 32 x 12288 x
 //    4096 with 48 columns rather 11.1 -> 12.4).
 //  * x comes from L2 once per workgroup, 4 to 16 times the weight's bytes, so the columns of a workgroup are as many as make one
 //    round of workgroups (64 x 22016 x 4096: 32 columns 33.6, 96 22.0, 128 25.0 of the first form).
-//  * Up to some 1000 rows such workgroups fill the chip better than tiles (509 x 4096 x 4096 on 256 x 128: 61).
+//  * Where one round of such workgroups (64 x 128 results on each of 256 CUs) holds all results they beat tiles, which then leave CUs idle;
+//    from the second round on tiles of 128 rows win (us, 64 x 128 here / the best tiles: 509 x 4096 x 4096 20.4 / 33.9, 800 x 4096 x 4096
+//    35.6 / 34.8, 1021 x 4096 x 4096 37.9 / 35.0, 509 x 12288 x 4096 59.6 / 49.5).
 #include "mx_tile.h"
 
 using namespace lumen;

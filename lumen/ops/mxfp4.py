@@ -199,8 +199,8 @@ def _decode(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 
 # What a round of 256 workgroups takes, us (bf16, weights from HBM), as a time a stage of 64 k and one beside them: a + b rt and f + g rt on the
-# few-row kernel's xr x 16 rt results, c and e on tiles of 32 mj x 32 ni (the kernels say what either form takes).  Over 210 sizes of 1 to
-# 4096 rows the form chosen takes 0.5 % more than the best one, 15 % at worst.
+# few-row kernel's xr x 16 rt results, c and e on tiles of 32 mj x 32 ni (the kernels say what either form takes).  Over 222 sizes of 1 to
+# 4096 rows, all three products, the form chosen takes 0.5 % more than the best of the seven that this predicts to be fastest, 12 % at worst.
 _ROWS = [(xr, 16 * rt, (0, xr, rt), a + b * rt, f + g * rt)
          for xr, a, b, f, g, rts in ((16, 0.03, 0.0075, 1.8, 0.4, (1, 2, 3, 4, 6, 8)), (32, 0.065, 0.012, 1.9, 0.5, (1, 2, 3, 4, 6)),
                                      (32, 0.21, 0.0, 5.0, 0.0, (8,)), (64, 0.09, 0.017, 2.3, 0.5, (2, 3, 4, 6, 8)))
