@@ -22,7 +22,7 @@
 //    output columns of one row: 8-byte stores;
 //  * split-K (S > 1) is reduced IN the launch: every slice writes its f32 slab, takes a ticket
 //    on the tile's counter (agent-scope release), and the last arriver (agent-scope acquire) sums
-//    the other slabs into its registers and stores the tile.  Slices of a tile are mapped to
+//    the slabs in the slices' order, its own from its registers, and stores the tile.  Slices of a tile are mapped to
 //    neighbouring virtual block ids under the XCD-aware remap, so they share an XCD.
 #include "common.h"
 
@@ -227,15 +227,26 @@ dgemm_kernel(const T* __restrict__ x, const T* __restrict__ W, T* __restrict__ y
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     __syncthreads();
+    // in the slices' order, whichever came last: the same bits every time
+    f32x4 sum[NI][MJ];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < MJ; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int o = 0; o < S; ++o) {
-      if (o == slice) continue;
       const float* os = ws + ((long long)tile * S + o) * (NT * NI * MJ * 4);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < MJ; ++j)
-          acc[i][j] += *reinterpret_cast<const f32x4*>(os + ((i * MJ + j) * NT + threadIdx.x) * 4);
+        for (int j = 0; j < MJ; ++j) {
+          if (o == slice) sum[i][j] += acc[i][j];
+          else sum[i][j] += *reinterpret_cast<const f32x4*>(os + ((i * MJ + j) * NT + threadIdx.x) * 4);
+        }
     }
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < MJ; ++j) acc[i][j] = sum[i][j];
   }
 
   // lane holds y^T[n = n0 + nrow0 + 16 i + 4 (lane >> 4) + 0..3][m = mrow0 - BN + 16 j + (lane & 15)]

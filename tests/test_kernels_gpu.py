@@ -969,6 +969,27 @@ def test_every_plan_of_the_table_is_one_that_linear_nt_runs():
             assert torch.equal(out, y) and torch.equal(gemm.linear_nt(x, w), y)
 
 
+@pytest.mark.parametrize("bm,bn,S,nw", [(256, 64, 3, 8), (256, 160, 4, 4), (128, 256, 3, 4), (64, 128, 3, 4)])
+def test_decode_gemm_adds_its_slices_in_order(bm, bn, S, nw):
+    """One product a slice, 2^24, 1, -2^24 (and -1) in every arrangement: fp32 sums of them differ with the order, so the result is that
+    of the slices' order only if no other is taken, whichever workgroup of a tile comes last."""
+    import itertools
+
+    from lumen.ops.gemm import decode_gemm
+
+    N, K, tiles = 2048, 1280, 20                          # (tiles of 64 k)
+    ends = [tiles // S * s + min(s, tiles % S) for s in range(S)]
+    for vals in itertools.permutations([2.0 ** 24, 1.0, -2.0 ** 24, -1.0][:S]):
+        x = torch.zeros(bm, K, device=DEV, dtype=torch.bfloat16)
+        w = torch.zeros(N, K, device=DEV, dtype=torch.bfloat16)
+        want = torch.zeros((), dtype=torch.float32)
+        for e, v in zip(ends, vals):
+            x[:, 64 * e], w[:, 64 * e] = (v if abs(v) == 1 else math.copysign(4096, v)), (1 if abs(v) == 1 else 4096)
+            want = want + torch.tensor(v, dtype=torch.float32)
+        wrong = sum(int((decode_gemm(x, w, bm, bn, S, nw).float() != float(want)).sum()) for _ in range(5))
+        assert wrong == 0, vals
+
+
 @pytest.mark.parametrize("N,F", [(4096, 11008), (1024, 2752)])
 def test_swiglu_down_projection(N, F):
     """Batch-1 MLP down projection of the serving path: SwiGLU kernel + weight-streaming GEMV ==
