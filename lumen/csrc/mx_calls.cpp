@@ -197,8 +197,8 @@ struct Product : torch::autograd::Node {
     const std::lock_guard<std::mutex> lock(mutex_);
     data.reset_data();
   }
-  // A leaf's accumulation node belongs to the stream of the first of its graphs that are alive.  If that stream is not the captured one,
-  // the engine makes it wait for the capture, which no capture survives (and an error there ends the process).
+  // A leaf's accumulation node belongs to the stream of the first of its graphs that are alive.  If that is the default stream, the engine
+  // makes it wait for the capture, which no capture survives (and an error there ends the process).
   void refuse_foreign_accumulation(const c10::Device& device) const {
     const auto ours = c10::hip::getCurrentHIPStream(device.index());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -208,8 +208,8 @@ struct Product : torch::autograd::Node {
     while (node && node->num_outputs() == 1) node = node->next_edge(0).function.get();       // (views of the leaf)
     auto* sum = dynamic_cast<torch::autograd::AccumulateGrad*>(node);
     const auto theirs = sum ? sum->stream() : std::nullopt;
-    TORCH_CHECK_VALUE(!theirs || theirs->id() == ours.id(), "gradient of mxfp4_linear: the captured pass ends at a leaf whose graph from "
-                      "before the capture is alive; drop that graph first");
+    TORCH_CHECK_VALUE(!theirs || theirs->id() != 0, "gradient of mxfp4_linear: the captured pass ends at a leaf whose graph from before the "
+                      "capture is alive on the default stream; drop that graph first");
   }
   std::string name() const override { return "Mxfp4LinearBackward"; }
 };
